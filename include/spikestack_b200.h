@@ -40,8 +40,9 @@ enum {
   SPK_EDEVICE = 5        /* a kernel reported a device-side error (spk_device_error) */
 };
 
-/* weight element types */
-enum { SPK_F32 = 0, SPK_BF16 = 1 };
+/* element types (weights: SPK_F32 or SPK_BF16; the training and streaming
+ * operators: all three) */
+enum { SPK_F32 = 0, SPK_BF16 = 1, SPK_F16 = 2 };
 
 /* spike-linear branch selection */
 enum {
@@ -191,7 +192,8 @@ int spk_sparse_multistep_forward(const float* dense_input, int T, int64_t B, int
  * fp32-accurate on the tensor cores (tf32 hi/lo splits of W and X).  Needs
  * N > 64, K % 4 == 0 and a 16-byte aligned X.  Replaces the nn.Linear +
  * threshold + Heaviside pairs around the spike-linear path. */
-enum { SPK_ACT_NONE = 0, SPK_ACT_HEAVISIDE = 1, SPK_ACT_VSPIKE = 2, SPK_ACT_HEAVISIDE_BITS = 3, SPK_ACT_VSPIKE_BITS = 4 };
+enum { SPK_ACT_NONE = 0, SPK_ACT_HEAVISIDE = 1, SPK_ACT_VSPIKE = 2, SPK_ACT_HEAVISIDE_BITS = 3, SPK_ACT_VSPIKE_BITS = 4,
+       SPK_ACT_SILU = 5 /* y sigmoid(y), group norm only */ };
 /* SPK_ACT_HEAVISIDE_BITS: the Heaviside spikes of SPK_ACT_HEAVISIDE packed one
  * bit each, Y read as uint32 [R][N/32] (bit b of word w of a row = column
  * 32w + b; N % 32 == 0): 32x fewer bytes than the fp32 spike tensor for the
@@ -313,6 +315,77 @@ int spk_spire_planes(const float* u, const float* frontier, const float* tempora
  * 16-byte aligned. */
 int spk_temporal_mean(const float* x, int T, int64_t B, int N, int d, float* mean_x, float* mean_spike,
                       spk_stream_t stream);
+
+/* ------------------------------------------------------- gated linear recurrence
+ * The linear counterpart of the GSMC recurrence over time, with its backward
+ * pass.  Per batch row b and channel d, for t = 0 .. len_b - 1, from the state
+ * h_{-1} = state[b, d] (0 when state is null):
+ *   SPK_REC_GATE   h_t = gate_t h_{t-1} + x_t
+ *   SPK_REC_LEAKY  h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(gate_t)
+ * x, gate and h hold dtype (SPK_F32, SPK_BF16 or SPK_F16); element (b, t, d) is
+ * at base + b*stride_b + t*stride_t + d, so time may be any dimension but the
+ * last and an input may be a slice or be broadcast (stride 0).  States are
+ * fp32 [B, D] contiguous: last = h_{len_b - 1} (the initial state for an
+ * empty row).  lengths [B] int32 (null: all L; values are clamped to [0, L]):
+ * inputs at t >= len_b are not read, and h is 0 there.  Non-finite inputs
+ * make the channel's later states non-finite.
+ * carry (optional, for the backward pass): fp32
+ * [ceil(L / spk_recurrence_chunk()) - 1, B, D], the states before each chunk
+ * but the first.  Arithmetic is fp32, h rounded once.  No reference
+ * counterpart (its GSMC loop, nn/gsmc.py:119-142, is nonlinear in the state
+ * and runs step by step). */
+enum { SPK_REC_GATE = 0, SPK_REC_LEAKY = 1 };
+int spk_recurrence_chunk(void);
+size_t spk_recurrence_workspace_bytes(int64_t B, int64_t L, int64_t D);
+int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate, int64_t g_stride_b,
+                   int64_t g_stride_t, int dtype, int form, int64_t B, int64_t L, int64_t D, const float* state,
+                   const int32_t* lengths, void* h, int64_t h_stride_b, int64_t h_stride_t, float* last,
+                   float* carry, void* workspace, size_t workspace_bytes, spk_stream_t stream);
+/* gh (null: zero) is the gradient of h, glast (null: zero) that of last; dx
+ * and dgate share their strides and are 0 at t >= len_b; dstate may be null.
+ * carry is the forward pass's (may be null for L <= spk_recurrence_chunk()). */
+int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate,
+                            int64_t g_stride_b, int64_t g_stride_t, const void* gh, int64_t gh_stride_b,
+                            int64_t gh_stride_t, int dtype, int form, int64_t B, int64_t L, int64_t D,
+                            const float* state, const int32_t* lengths, const float* carry, const float* glast,
+                            void* dx, void* dgate, int64_t d_stride_b, int64_t d_stride_t, float* dstate,
+                            void* workspace, size_t workspace_bytes, spk_stream_t stream);
+/* One step over n cells (all contiguous): out [n] dtype, new_state [n] fp32
+ * (may be state itself). */
+int spk_recurrence_step(const void* x, const void* gate, int dtype, int form, int64_t n, const float* state,
+                        void* out, float* new_state, spk_stream_t stream);
+
+/* ------------------------------------------------------- group norm + activation
+ * Group norm on channels-last X [S, P, C] with act SPK_ACT_NONE,
+ * SPK_ACT_HEAVISIDE (1 if z - thr > 0 else 0) or SPK_ACT_SILU: per sample and
+ * group of C / G channels, over P * C / G elements, the biased variance, then
+ * z = (x - mean) rstd weight[c] + bias[c], Y = act(z).  X and Y hold dtype;
+ * weight, bias (null: 1, 0), mean and rstd [S, G] (outputs, both or neither
+ * null) are fp32.  No reference counterpart (its blocks use layer norm). */
+size_t spk_group_norm_workspace_bytes(int64_t S, int64_t P, int C, int G);
+int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P, int C, int G, const float* weight,
+                       const float* bias, float eps, int act, float thr, void* Y, float* mean, float* rstd,
+                       void* workspace, size_t workspace_bytes, spk_stream_t stream);
+/* Gradients from GY = dL/dY and the forward pass's mean and rstd: DX (dtype),
+ * dweight and dbias (fp32 [C], may be null; the same bits on every run).  The
+ * Heaviside's derivative is the sigmoid surrogate of the reference's spike_fn
+ * (nn/attention.py:13-24). */
+int spk_group_norm_act_backward(const void* X, const void* GY, int dtype, int64_t S, int64_t P, int C, int G,
+                                const float* weight, const float* bias, const float* mean, const float* rstd,
+                                int act, float thr, void* DX, float* dweight, float* dbias, void* workspace,
+                                size_t workspace_bytes, spk_stream_t stream);
+
+/* ------------------------------------------------------- dropout
+ * Y[i] = (R ? R[i] : 0) + (w_i >= round(p 2^32) ? X[i] / (1 - p) : 0) over n
+ * elements of dtype, where w_i is word i % 4 of Philox4x32 with 7 rounds at
+ * counter (i / 4, offset) under the key `seed` (64-bit numbers as two words,
+ * low first).  key (optional, device memory): {seed, offset}, read by the
+ * kernel in place of the two arguments, so that a captured graph can be given
+ * new numbers.  The mask is never stored: the backward pass is this call on
+ * the gradient, R null.  Y may be X or R.  A dropped element contributes 0
+ * whatever it holds. */
+int spk_dropout(const void* X, const void* R, int dtype, int64_t n, double p, uint64_t seed, uint64_t offset,
+                const int64_t* key, void* Y, spk_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libspk_b200.so")
 
 SPK_OK, SPK_EINVAL, SPK_EUNSUPPORTED, SPK_ECUDA, SPK_EWORKSPACE, SPK_EDEVICE = range(6)
-SPK_F32, SPK_BF16 = 0, 1
+SPK_F32, SPK_BF16, SPK_F16 = 0, 1, 2
 # device error bits (spk_device_error)
 SPK_DEV_PIPE_TIMEOUT, SPK_DEV_SCAN_TIMEOUT, SPK_DEV_CSR_OVERFLOW, SPK_DEV_TMEM = 1, 2, 4, 8
 BRANCH_AUTO, BRANCH_DENSE, BRANCH_CSR = 0, 1, 2
@@ -61,6 +61,16 @@ SIGNATURES = {
     "spk_selftest_wait_timeout": (_I, [_P]),
     "spk_spire_planes": (_I, [_P, _P, _P, _P, _I, _L, _I, _I, _P, _P]),
     "spk_temporal_mean": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
+    "spk_recurrence_chunk": (_I, []),
+    "spk_recurrence_workspace_bytes": (_Z, [_L, _L, _L]),
+    "spk_recurrence": (_I, [_P, _L, _L, _P, _L, _L, _I, _I, _L, _L, _L, _P, _P, _P, _L, _L, _P, _P, _P, _Z, _P]),
+    "spk_recurrence_backward": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P,
+                                     _L, _L, _P, _P, _Z, _P]),
+    "spk_recurrence_step": (_I, [_P, _P, _I, _I, _L, _P, _P, _P, _P]),
+    "spk_group_norm_workspace_bytes": (_Z, [_L, _L, _I, _I]),
+    "spk_group_norm_act": (_I, [_P, _I, _L, _L, _I, _I, _P, _P, _F, _I, _F, _P, _P, _P, _P, _Z, _P]),
+    "spk_group_norm_act_backward": (_I, [_P, _P, _I, _L, _L, _I, _I, _P, _P, _P, _P, _I, _F, _P, _P, _P, _P, _Z, _P]),
+    "spk_dropout": (_I, [_P, _P, _I, _L, _c.c_double, _c.c_uint64, _c.c_uint64, _P, _P, _P]),
 }
 
 _lib = None

@@ -1,0 +1,70 @@
+// Element types of the training and streaming operators: fp32, bf16 and fp16
+// tensors whose arithmetic is fp32, rounded once (to nearest even) when an
+// output is stored.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "spk_common.cuh"
+
+namespace spk {
+
+__device__ __forceinline__ float elem_to_f32(float v) { return v; }
+__device__ __forceinline__ float elem_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float elem_to_f32(__half v) { return __half2float(v); }
+
+template <typename E>
+__device__ __forceinline__ E elem_from_f32(float v);
+template <>
+__device__ __forceinline__ float elem_from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 elem_from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half elem_from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// V consecutive elements moved as one access (V * sizeof(E) <= 16 bytes, the
+// address a multiple of that).
+template <typename E, int V>
+struct alignas(sizeof(E) * V) Pack {
+  E e[V];
+};
+
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> load_pack(const E* p) {
+  return *reinterpret_cast<const Pack<E, V>*>(p);
+}
+template <typename E, int V>
+__device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& v) {
+  *reinterpret_cast<Pack<E, V>*>(p) = v;
+}
+
+inline size_t elem_bytes(int dtype) { return dtype == SPK_F32 ? 4 : (dtype == SPK_BF16 || dtype == SPK_F16) ? 2 : 0; }
+
+inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// Calls f with a value of the element type (dispatch on dtype); false for an
+// unknown dtype.
+template <typename F>
+inline bool with_elem(int dtype, F&& f) {
+  switch (dtype) {
+    case SPK_F32:
+      f(float{});
+      return true;
+    case SPK_BF16:
+      f(__nv_bfloat16{});
+      return true;
+    case SPK_F16:
+      f(__half{});
+      return true;
+    default:
+      return false;
+  }
+}
+
+}  // namespace spk

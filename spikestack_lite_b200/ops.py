@@ -572,3 +572,350 @@ def temporal_mean(x):
     check(_lib.load().spk_temporal_mean(ptr(x), T, B, N, d, ptr(mean_x), ptr(mean_s), stream_of(x)),
           "spk_temporal_mean")
     return mean_x, mean_s
+
+
+# --------------------------------------------------------------------------- training and streaming operators
+# The operators below take float32, bfloat16 or float16 tensors (fp32
+# arithmetic, results rounded once) and are differentiable.  Scratch memory is
+# allocated per call, so calls on several streams and captured graphs never
+# share any.
+_DTYPES = {torch.float32: _lib.SPK_F32, torch.bfloat16: _lib.SPK_BF16, torch.float16: _lib.SPK_F16}
+
+
+def _dtype(t, what):
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise EngineError(f"{what}: float32, bfloat16 or float16 tensors required, got {t.dtype}") from None
+
+
+def _same_device(t, *others, what):
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise EngineError(f"{what}: tensors on {t.device} and {o.device}")
+
+
+def _call(t, name, *args):
+    """Entry point `name` on t's device and its current stream (the last argument)."""
+    fn = getattr(_lib.load(), name)
+    if t.device.index == torch.cuda.current_device():
+        check(fn(*args, stream_of(t)), name)
+    else:
+        with torch.cuda.device(t.device):
+            check(fn(*args, stream_of(t)), name)
+
+
+def _scratch(t, nbytes):
+    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------- gated linear recurrence
+_FORMS = {"gate": 0, "leaky": 1}
+
+
+def _form(form, what):
+    try:
+        return _FORMS[form]
+    except (KeyError, TypeError):
+        raise EngineError(f"{what}: form must be one of {sorted(_FORMS)}, got {form!r}") from None
+
+
+def _time_strides(t, dim):
+    """(stride of the flattened batch, stride of time) of t with time at
+    dimension `dim` and every other dimension but the last one batch; None when
+    the batch dimensions do not flatten or the last one is not contiguous."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return None
+    step, size = None, 1
+    for i in range(t.dim() - 2, -1, -1):  # from the innermost batch dimension outwards
+        if i == dim or t.shape[i] == 1:
+            continue
+        if step is None:
+            step, size = t.stride(i), t.shape[i]
+        elif t.stride(i) != step * size:
+            return None
+        else:
+            size *= t.shape[i]
+    return (step if step is not None else 0), t.stride(dim)
+
+
+def _time_major(t, dim):
+    """t itself, or a copy, such that _time_strides(result, dim') holds, and dim'."""
+    st = _time_strides(t, dim)
+    if st is not None:
+        return t, st
+    t = t.movedim(dim, -2).contiguous().movedim(-2, dim)
+    return t, _time_strides(t, dim)
+
+
+def _empty_time(t, dim):
+    """An uninitialised tensor of t's shape whose batch dimensions flatten, and its strides."""
+    out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return _time_major(out, dim) if out.numel() else (out, (0, 0))
+
+
+def _recurrence_forward(x, gate, state, form, dim, lengths, keep):
+    """(h, last, carry) through spk_recurrence; `keep`: fill carry for the backward pass."""
+    lib = _lib.load()
+    L, D = x.shape[dim], x.shape[-1]
+    B = x.numel() // (L * D) if x.numel() else (state.numel() // D if D else 0)
+    (x, (xb, xt)), (gate, (gb, gt)), (h, (hb, ht)) = _time_major(x, dim), _time_major(gate, dim), _empty_time(x, dim)
+    last = torch.empty_like(state)
+    chunk = int(lib.spk_recurrence_chunk())
+    carry = None
+    if keep and L > chunk:
+        carry = torch.empty((L + chunk - 1) // chunk - 1, B, D, dtype=torch.float32, device=x.device)
+    ws = _scratch(x, lib.spk_recurrence_workspace_bytes(B, L, D))
+    _call(x, "spk_recurrence", ptr(x), xb, xt, ptr(gate), gb, gt, _DTYPES[x.dtype], form, B, L, D, ptr(state),
+          ptr(lengths), ptr(h), hb, ht, ptr(last), ptr(carry), ptr(ws), 0 if ws is None else ws.numel())
+    return h, last, carry
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, state, form, dim, lengths):
+        h, last, carry = _recurrence_forward(x, gate, state, form, dim, lengths, True)
+        ctx.save_for_backward(x, gate, state, lengths, carry)
+        ctx.form, ctx.dim = form, dim
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gh, glast):
+        x, gate, state, lengths, carry = ctx.saved_tensors
+        if gh is None and glast is None:
+            return (None,) * 6
+        dim, lib = ctx.dim, _lib.load()
+        L, D = x.shape[dim], x.shape[-1]
+        B = state.numel() // D if D else 0
+        (x, (xb, xt)), (gate, (gb, gt)) = _time_major(x, dim), _time_major(gate, dim)
+        ghb = ght = 0
+        if gh is not None:
+            gh, (ghb, ght) = _time_major(gh, dim)
+        glast = None if glast is None else _contig(glast)
+        dx, (db, dt) = _empty_time(x, dim)
+        dgate, _ = _empty_time(x, dim)
+        dstate = torch.empty_like(state)
+        ws = _scratch(x, lib.spk_recurrence_workspace_bytes(B, L, D))
+        _call(x, "spk_recurrence_backward", ptr(x), xb, xt, ptr(gate), gb, gt, ptr(gh), ghb, ght, _DTYPES[x.dtype],
+              ctx.form, B, L, D, ptr(state), ptr(lengths), ptr(carry), ptr(glast), ptr(dx), ptr(dgate), db, dt,
+              ptr(dstate), ptr(ws), 0 if ws is None else ws.numel())
+        return dx, dgate, dstate, None, None, None
+
+
+def gated_recurrence(x, gate, state=None, form="leaky", dim=-2, lengths=None):
+    """Gated linear recurrence along dimension `dim` of x [..., d] (any but the
+    last), with gate of x's shape and dtype (spk_recurrence):
+
+      "leaky"  h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(gate_t)
+      "gate"   h_t = gate_t h_{t-1} + x_t
+
+    from `state` (float32, x's shape without `dim`; None: zero).  Returns (h,
+    last): h like x, last the float32 state after the last step, to be handed
+    to the next call or to gated_recurrence_step.  ``lengths`` (int32 or int64,
+    x's shape without `dim` and the last dimension; clamped to [0, steps]):
+    steps at or beyond a row's length are not read, h is 0 there and the state
+    stays.  x and gate may be slices or broadcast views whose last dimension is
+    contiguous.  Differentiable in x, gate and state."""
+    what = "gated_recurrence"
+    require_cuda(x, gate, state, lengths, what=what)
+    form = _form(form, what)
+    _dtype(x, what)
+    _same_device(x, gate, state, lengths, what=what)
+    if gate.dtype != x.dtype or gate.shape != x.shape:
+        raise EngineError(f"{what}: gate must have x's shape and dtype ({tuple(x.shape)}, {x.dtype}), "
+                          f"got {tuple(gate.shape)}, {gate.dtype}")
+    if x.dim() < 2 or not -x.dim() <= dim < x.dim() or dim % x.dim() == x.dim() - 1:
+        raise EngineError(f"{what}: dim must name a dimension of x but the last, got {dim} for {tuple(x.shape)}")
+    dim %= x.dim()
+    shape = x.shape[:dim] + x.shape[dim + 1:]
+    if state is None:
+        state = torch.zeros(shape, dtype=torch.float32, device=x.device)
+    elif state.dtype != torch.float32 or state.shape != shape:
+        raise EngineError(f"{what}: state must be float32 of shape {tuple(shape)}, got {tuple(state.shape)}, "
+                          f"{state.dtype}")
+    if lengths is not None:
+        if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != shape[:-1]:
+            raise EngineError(f"{what}: lengths must be int32 or int64 of shape {tuple(shape[:-1])}, got "
+                              f"{tuple(lengths.shape)}, {lengths.dtype}")
+        if lengths.dtype == torch.int64:  # clamped first: the cast wraps
+            lengths = lengths.clamp(0, x.shape[dim]).to(torch.int32)
+        lengths = _contig(lengths)
+    state = _contig(state)
+    if _wants_grad(x, gate, state):
+        return _GatedRecurrence.apply(x, gate, state, form, dim, lengths)
+    return _recurrence_forward(x, gate, state, form, dim, lengths, False)[:2]
+
+
+def gated_recurrence_step(x, gate, state, form="leaky", new_state=None):
+    """One step of gated_recurrence for streaming: x and gate [..., d] of one
+    time step, state float32 of the same shape -> (h, new state): h in x's
+    dtype, the state in float32.  ``new_state``: the tensor to write it to
+    (contiguous float32; `state` itself updates it in place).  Not
+    differentiable."""
+    what = "gated_recurrence_step"
+    require_cuda(x, gate, state, new_state, what=what)
+    form = _form(form, what)
+    dt = _dtype(x, what)
+    _same_device(x, gate, state, new_state, what=what)
+    if gate.dtype != x.dtype or gate.shape != x.shape:
+        raise EngineError(f"{what}: gate must have x's shape and dtype")
+    if state.dtype != torch.float32 or state.shape != x.shape:
+        raise EngineError(f"{what}: state must be float32 of x's shape {tuple(x.shape)}")
+    if _wants_grad(x, gate, state):
+        raise EngineError(f"{what}: no backward pass (use gated_recurrence, or torch.no_grad())")
+    if new_state is None:
+        new_state = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    elif new_state.dtype != torch.float32 or new_state.shape != x.shape or not new_state.is_contiguous():
+        raise EngineError(f"{what}: new_state must be contiguous float32 of x's shape {tuple(x.shape)}")
+    x, gate, state = _contig(x), _contig(gate), _contig(state)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _call(x, "spk_recurrence_step", ptr(x), ptr(gate), dt, form, x.numel(), ptr(state), ptr(out), ptr(new_state))
+    return out, new_state
+
+
+# ------------------------------------------------------------- group norm + activation
+_NORM_ACTS = {"none": 0, "heaviside": 1, "silu": 5}
+
+
+def _group_norm_forward(x, groups, weight, bias, eps, act, thr, keep):
+    """(y, mean, rstd) through spk_group_norm_act; mean and rstd [S, G] when `keep`."""
+    lib = _lib.load()
+    S, C = x.shape[0], x.shape[-1]
+    P = x[0].numel() // C if S else 0
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(S, groups, dtype=torch.float32, device=x.device) if keep else None
+    rstd = torch.empty_like(mean) if keep else None
+    ws = _scratch(x, lib.spk_group_norm_workspace_bytes(S, P, C, groups))
+    _call(x, "spk_group_norm_act", ptr(x), _DTYPES[x.dtype], S, P, C, groups, ptr(weight), ptr(bias), eps, act, thr,
+          ptr(y), ptr(mean), ptr(rstd), ptr(ws), 0 if ws is None else ws.numel())
+    return y, mean, rstd
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, thr):
+        y, mean, rstd = _group_norm_forward(x, groups, weight, bias, eps, act, thr, True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.groups, ctx.act, ctx.thr = groups, act, thr
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        lib = _lib.load()
+        gy = _contig(gy)
+        S, C = x.shape[0], x.shape[-1]
+        P = x[0].numel() // C if S else 0
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dweight = torch.empty(C, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[1] else None
+        dbias = torch.empty(C, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
+        ws = _scratch(x, lib.spk_group_norm_workspace_bytes(S, P, C, ctx.groups))
+        _call(x, "spk_group_norm_act_backward", ptr(x), ptr(gy), _DTYPES[x.dtype], S, P, C, ctx.groups, ptr(weight),
+              ptr(bias), ptr(mean), ptr(rstd), ctx.act, ctx.thr, ptr(dx), ptr(dweight), ptr(dbias), ptr(ws),
+              0 if ws is None else ws.numel())
+        return dx, dweight, dbias, None, None, None, None
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", thr=0.0):
+    """act(group norm of x) for channels-last x [S, ..., C] (spk_group_norm_act):
+    per sample (the first dimension) and group of C / groups neighbouring
+    channels, normalised over all positions in between, then scaled by weight
+    [C] and shifted by bias [C] (float32; None: 1 / 0), then
+
+      "none"       z
+      "silu"       z sigmoid(z)
+      "heaviside"  (z - thr > 0), with spike_fn's surrogate gradient
+
+    A (T, B, N, d) tensor is normalised per time plane and sample as
+    x.flatten(0, 1).  Differentiable in x, weight and bias."""
+    what = "group_norm_act"
+    require_cuda(x, weight, bias, what=what)
+    require_f32(weight, bias, what=what)
+    _dtype(x, what)
+    _same_device(x, weight, bias, what=what)
+    if act not in _NORM_ACTS:
+        raise EngineError(f"{what}: act must be one of {sorted(_NORM_ACTS)}")
+    if x.dim() < 2 or x.shape[-1] == 0:
+        raise EngineError(f"{what}: x must be (samples, ..., channels), got {tuple(x.shape)}")
+    C, groups = x.shape[-1], int(groups)
+    if groups < 1 or C % groups:
+        raise EngineError(f"{what}: {C} channels do not form {groups} groups")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and p.shape != (C,):
+            raise EngineError(f"{what}: {name} must have shape ({C},), got {tuple(p.shape)}")
+    x = _contig(x)
+    weight = None if weight is None else _contig(weight)
+    bias = None if bias is None else _contig(bias)
+    if _wants_grad(x, weight, bias):
+        return _GroupNormAct.apply(x, weight, bias, groups, float(eps), _NORM_ACTS[act], float(thr))
+    return _group_norm_forward(x, groups, weight, bias, float(eps), _NORM_ACTS[act], float(thr), False)[0]
+
+
+# ------------------------------------------------------------- dropout
+def _dropout_call(x, residual, p, key):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dev = key if isinstance(key, torch.Tensor) else None
+    seed, offset = (0, 0) if dev is not None else key
+    _call(x, "spk_dropout", ptr(x), ptr(residual), _DTYPES[x.dtype], x.numel(), p, seed, offset, ptr(dev), ptr(y))
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, key):
+        ctx.p = p
+        ctx.key = None if isinstance(key, torch.Tensor) else key
+        ctx.save_for_backward(key if ctx.key is None else None)
+        return _dropout_call(x, residual, p, key)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        key = ctx.saved_tensors[0] if ctx.key is None else ctx.key
+        gx = _dropout_call(_contig(gy), None, ctx.p, key) if ctx.needs_input_grad[0] else None
+        return gx, (gy if ctx.needs_input_grad[1] else None), None, None
+
+
+def dropout(x, p, key, residual=None):
+    """Dropout with the residual added: residual + keep * x / (1 - p)
+    (spk_dropout).  The mask is a function of `key` = (seed, offset) and the
+    element's index in x -- a counter-based generator -- and is never stored:
+    the backward pass makes it again.  ``key``: two Python integers, or an
+    int64 CUDA tensor of two elements, read by the kernel, so that a captured
+    graph takes new numbers when the tensor is changed (it must keep its value
+    from the forward to the backward pass).  Give every call of a step its own
+    offset.  Differentiable in x and residual."""
+    what = "dropout"
+    require_cuda(x, residual, what=what)
+    _dtype(x, what)
+    _same_device(x, residual, what=what)
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise EngineError(f"{what}: p must lie in [0, 1], got {p}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise EngineError(f"{what}: residual must have x's shape and dtype ({tuple(x.shape)}, {x.dtype}), "
+                          f"got {tuple(residual.shape)}, {residual.dtype}")
+    if isinstance(key, torch.Tensor):
+        require_cuda(key, what=what)
+        _same_device(x, key, what=what)
+        if key.dtype != torch.int64 or key.shape != (2,):
+            raise EngineError(f"{what}: key must be int64 of shape (2,), got {tuple(key.shape)}, {key.dtype}")
+        key = _contig(key)
+    else:
+        try:
+            seed, offset = (int(v) & 0xFFFFFFFFFFFFFFFF for v in key)
+        except (TypeError, ValueError):
+            raise EngineError(f"{what}: key must be two integers or an int64 CUDA tensor") from None
+        key = (seed, offset)
+    x = _contig(x)
+    residual = None if residual is None else _contig(residual)
+    if _wants_grad(x, residual):
+        return _Dropout.apply(x, residual, p, key)
+    return _dropout_call(x, residual, p, key)
