@@ -327,29 +327,28 @@ int spk_temporal_mean(const float* x, int T, int64_t B, int N, int d, float* mea
  * last and an input may be a slice or be broadcast (stride 0).  States are
  * fp32 [B, D] contiguous: last = h_{len_b - 1} (the initial state for an
  * empty row).  lengths [B] int32 (null: all L; values are clamped to [0, L]):
- * inputs at t >= len_b are not read, and h is 0 there.  Non-finite inputs
- * make the channel's later states non-finite.
+ * inputs at t >= len_b are not read, and h is 0 there.  A NaN, or an
+ * infinite x, makes the channel's later states non-finite.
  * carry (optional, for the backward pass): fp32
- * [ceil(L / spk_recurrence_chunk()) - 1, B, D], the states before each chunk
- * but the first.  Arithmetic is fp32, h rounded once.  No reference
+ * [ceil(L / C) - 1, B, D] with C = spk_recurrence_chunk(B, L, D), the states
+ * before each chunk of C steps but the first.  Arithmetic is fp32, h rounded once.  No reference
  * counterpart (its GSMC loop, nn/gsmc.py:119-142, is nonlinear in the state
  * and runs step by step). */
 enum { SPK_REC_GATE = 0, SPK_REC_LEAKY = 1 };
-int spk_recurrence_chunk(void);
-size_t spk_recurrence_workspace_bytes(int64_t B, int64_t L, int64_t D);
+int64_t spk_recurrence_chunk(int64_t B, int64_t L, int64_t D);
 int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate, int64_t g_stride_b,
                    int64_t g_stride_t, int dtype, int form, int64_t B, int64_t L, int64_t D, const float* state,
                    const int32_t* lengths, void* h, int64_t h_stride_b, int64_t h_stride_t, float* last,
-                   float* carry, void* workspace, size_t workspace_bytes, spk_stream_t stream);
+                   float* carry, spk_stream_t stream);
 /* gh (null: zero) is the gradient of h, glast (null: zero) that of last; dx
  * and dgate share their strides and are 0 at t >= len_b; dstate may be null.
- * carry is the forward pass's (may be null for L <= spk_recurrence_chunk()). */
+ * carry is the forward pass's (may be null when one chunk holds all steps). */
 int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate,
                             int64_t g_stride_b, int64_t g_stride_t, const void* gh, int64_t gh_stride_b,
                             int64_t gh_stride_t, int dtype, int form, int64_t B, int64_t L, int64_t D,
                             const float* state, const int32_t* lengths, const float* carry, const float* glast,
                             void* dx, void* dgate, int64_t d_stride_b, int64_t d_stride_t, float* dstate,
-                            void* workspace, size_t workspace_bytes, spk_stream_t stream);
+                            spk_stream_t stream);
 /* One step over n cells (all contiguous): out [n] dtype, new_state [n] fp32
  * (may be state itself). */
 int spk_recurrence_step(const void* x, const void* gate, int dtype, int form, int64_t n, const float* state,

@@ -5,6 +5,8 @@
 
 #include <cuda_fp16.h>
 
+#include <mutex>
+
 #include "spk_common.cuh"
 
 namespace spk {
@@ -66,5 +68,32 @@ inline bool with_elem(int dtype, F&& f) {
       return false;
   }
 }
+
+// A value worked out once per device (the current one) and kept.
+template <typename T>
+class PerDevice {
+ public:
+  template <typename F>
+  cudaError_t get(T* out, F&& make) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= kDevices) return make(out);
+    std::lock_guard<std::mutex> lk(mu_);
+    if (!known_[dev]) {
+      e = make(&value_[dev]);
+      if (e != cudaSuccess) return e;
+      known_[dev] = true;
+    }
+    *out = value_[dev];
+    return cudaSuccess;
+  }
+
+ private:
+  static constexpr int kDevices = 64;
+  std::mutex mu_;
+  bool known_[kDevices] = {};
+  T value_[kDevices];
+};
 
 }  // namespace spk

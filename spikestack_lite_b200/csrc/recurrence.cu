@@ -22,7 +22,7 @@ struct RecArgs {
   const int32_t* lengths; // [B] or null
   void* h;
   float* last;            // [B, D]
-  float* carry;           // [chunks - 1, B, D]: the state before steps 64, 128, ...; or null
+  float* carry;           // [chunks - 1, B, D]: the states between tiles along time; or null
   void* dx;
   void* dgate;
   float* dh0;
@@ -30,15 +30,25 @@ struct RecArgs {
   int64_t x_b, x_t, g_b, g_t, h_b, h_t, o_b, o_t;  // strides in elements (h: h or gh; o: dx and dgate)
 };
 
+struct RecPlan {
+  int64_t chains, groups;  // chains = B * groups of neighbouring channels
+  int64_t tiles, chunks;   // blocks' tiles (short), tiles along time (long)
+  int wt, cols;            // warps along time (short); channels per chain
+};
+
 // The decay of one or more steps as one float per form: `coeff` from the gate,
 // `step` the new state, `apply` A h + H for a joined decay A, `join` the decay
 // of two in a row, `back` the gradient that passes a step, dx and dgate the
 // gradients of its inputs (dgate from grad_base of the state before and x).
+// A warp's steps are joined by `open`, one `more` per step and `close`.
 // kept_gate is the gate, kept the decay, of a step that keeps the state.
 struct GateForm {
   __device__ static float kept_gate() { return 1.0f; }
   __device__ static float kept() { return 1.0f; }
-  __device__ static float coeff(float gate) { return gate; }
+  __device__ static float open() { return 1.0f; }
+  __device__ static float coeff(float gate, float* = nullptr) { return gate; }
+  __device__ static float more(float acc, float a, float) { return acc * a; }
+  __device__ static float close(float acc) { return acc; }
   __device__ static float step(float h, float a, float x) { return fmaf(a, h, x); }
   __device__ static float apply(float a, float h, float H) { return fmaf(a, h, H); }
   __device__ static float join(float a, float b) { return a * b; }
@@ -48,22 +58,55 @@ struct GateForm {
   __device__ static float dgate(float g, float, float base) { return g * base; }
 };
 
-// Leaky form: whichever of a and q = 1 - a is at most one half, its sign bit
-// set when it is a.  Both ends of the gate keep their relative accuracy: a
-// slow channel's q and a fast channel's a are never differences from 1, and
-// neither are those of joined steps.
+__device__ __forceinline__ float ex2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float min_nan(float x, float y) {  // NaN when either is
+  float z;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+__device__ __forceinline__ float rcp_fast(float x) {  // of a normal number with a normal reciprocal
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Leaky form.  Joined decays are whichever of A and Q = 1 - A is at most one
+// half, the sign bit set when it is A: neither a slow channel's Q nor a fast
+// channel's A is a difference from 1.  Over a warp's steps, with e =
+// exp(-gate) and a = 1 / (1 + e), the product of decays is 1 / (1 + E) with
+// E = prod (1 + e) - 1, a sum of positive terms (kept finite: below 2^-124 a
+// joined decay is as good as 0).
+// The decay of one step is kept the same way for fp32 tensors (FINE).  For
+// 16-bit ones it is q itself, and exp is the hardware's: a fast channel's
+// result is then off by a rounding of the state before it and the weights by
+// some 2^-21, far below the 2^-9 or 2^-12 that its inputs and outputs carry,
+// for 16 instead of 33 instructions per element (the 16-bit kernels are
+// bound by instruction issue, the fp32 ones by memory).
+template <bool FINE>
 struct LeakyForm {
   __device__ static float kept_gate() { return __int_as_float(0x7f800000); }  // q = 0
   __device__ static float kept() { return 0.0f; }
-  __device__ static float coeff(float gate) {
-    const float e = expf(-fabsf(gate));
-    return copysignf(__fdividef(e, 1.0f + e), gate);
-  }
+  __device__ static float open() { return 0.0f; }
   __device__ static bool is_a(float c) { return __float_as_int(c) < 0; }
-  __device__ static float step(float h, float c, float x) {
-    const bool fast = is_a(c);  // x + a (h - x), else h + q (x - h)
-    const float base = fast ? x : h;
-    return fmaf(fabsf(c), (fast ? h : x) - base, base);
+  // the decay of a step; *e (when wanted) becomes exp(-gate)
+  __device__ static float coeff(float gate, float* e = nullptr) {
+    if (!FINE) {
+      const float ex = ex2_fast(min_nan(gate * -1.4426950409f, 124.0f));
+      if (e != nullptr) *e = ex;
+      return ex * rcp_fast(1.0f + ex);
+    }
+    const float small = expf(-fabsf(gate));
+    if (e != nullptr) *e = gate < 0.0f ? rcp_fast(fmaxf(small, 0x1p-124f)) : small;
+    return copysignf(small * rcp_fast(1.0f + small), gate);
+  }
+  __device__ static float more(float acc, float, float e) { return fminf(fmaf(acc, e, acc + e), 0x1p124f); }
+  __device__ static float close(float acc) {
+    const float a = rcp_fast(1.0f + acc);
+    return acc <= 1.0f ? acc * a : -a;
   }
   __device__ static float apply(float c, float h, float H) {
     return is_a(c) ? fmaf(-c, h, H) : fmaf(-c, h, h) + H;
@@ -75,11 +118,17 @@ struct LeakyForm {
     }
     return -((is_a(c) ? -c : 1.0f - c) * (is_a(d) ? -d : 1.0f - d));
   }
-  __device__ static float back(float g, float c) { return is_a(c) ? -c * g : fmaf(-c, g, g); }
-  __device__ static float dx(float g, float c) { return is_a(c) ? fmaf(c, g, g) : c * g; }
+  __device__ static float step(float h, float c, float x) {
+    if (!FINE) return fmaf(c, x - h, h);
+    const bool fast = is_a(c);  // x + a (h - x), else h + q (x - h)
+    const float base = fast ? x : h;
+    return fmaf(fabsf(c), (fast ? h : x) - base, base);
+  }
+  __device__ static float back(float g, float c) { return FINE && is_a(c) ? -c * g : fmaf(-c, g, g); }
+  __device__ static float dx(float g, float c) { return FINE && is_a(c) ? fmaf(c, g, g) : c * g; }
   __device__ static float grad_base(float h, float x) { return h - x; }
   __device__ static float dgate(float g, float c, float base) {
-    const float s = fabsf(c);
+    const float s = FINE ? fabsf(c) : c;
     return g * base * fmaf(-s, s, s);
   }
 };
@@ -91,395 +140,580 @@ __device__ __forceinline__ int64_t rec_len(const RecArgs& a, int64_t b) {
 }
 
 // ---- tiles
-// A tile is up to 64 steps of 128 neighbouring channels of one batch row (one
-// "chain" of tiles along time).  A warp holds 8 steps of it in registers, a
-// lane 4 channels; a block is 8 warps, `wt` of them along time (8 when there
-// are more than 32 steps) and 8 / wt along chains.  Each warp reduces its
-// steps to one affine map h -> A h + H, the warps' maps meet in shared memory,
-// and every warp then runs its steps once more from its own start, in the
-// order of the definition.
-//
-// More than 64 steps: the tiles of a chain are joined in the same launch.  A
-// block takes the next tile in time-major order (a ticket, so every tile it
-// may wait for has been taken already), publishes its map, looks back over its
-// predecessors' maps to the nearest finished state, and publishes the state
-// behind itself: x and gate are read once however few chains there are.
-constexpr int kRecSteps = 8;                      // steps per warp
-constexpr int kRecWarps = 8;                      // warps per block
-constexpr int kRecCols = 128;                     // channels per warp: 4 per lane
-constexpr int kRecChunk = kRecSteps * kRecWarps;  // steps per tile, and between the states kept for the backward pass
+// A warp holds S steps of 32 V neighbouring channels of one batch row (a
+// "chain" along time) in registers, V channels per lane, and a block is 8
+// warps.  Each warp reduces its steps to one affine map h -> A h + H, the maps
+// meet in shared memory, and every warp then runs its steps once more from its
+// own start, in the order of the definition: states are exact in the sense of
+// the sequential recurrence within a warp's steps, and joined by A h + H
+// between.  Blocks go from tile to tile: while one is worked on, the next
+// one's inputs are on their way to shared memory (each lane copies what it
+// will read itself, so that needs no barrier), 2 blocks per SM.
+constexpr int kRecWarps = 8;
+constexpr int kRecThreads = 32 * kRecWarps;
+constexpr int kRecMaxCluster = 16;
 
-struct RecPlan {
-  int64_t chains, groups;  // chains = B * groups of 128 channels
-  int64_t tiles;           // blocks
-  int chunks, wt;
-  uint32_t* ticket;        // followed by one flag per tile; null with one chunk
-  float* maps;             // [tiles][2][128]: A, H
-  float* states;           // [tiles][128]: the state behind the tile
+// The lane's V channels of `n` (at most 32 V) starting at p: neighbours moved
+// as one access (ALIGNED), or every 32nd.
+template <int V>
+struct Cols {
+  float v[V];
 };
 
-struct Quad {
-  float v[4];
-};
-
-// The lane's 4 channels of `n` (at most 128) starting at p: neighbours with
-// one access (ALIGNED), or every 32nd.
-template <bool ALIGNED>
+template <int V, bool ALIGNED>
 __device__ __forceinline__ int rec_col(int lane, int i) {
-  return ALIGNED ? 4 * lane + i : lane + 32 * i;
+  return ALIGNED ? V * lane + i : lane + 32 * i;
 }
 
-template <bool ALIGNED, typename E>
-__device__ __forceinline__ Quad rec_load(const E* p, int lane, int n, float other) {
-  Quad q;
+template <int V, bool ALIGNED, typename E>
+__device__ __forceinline__ Cols<V> rec_load(const E* p, int lane, int n, float other) {
+  Cols<V> q;
   if (ALIGNED) {
-    if (4 * lane < n) {
-      const Pack<E, 4> e = load_pack<E, 4>(p + 4 * lane);
+    if (V * lane < n) {
+      const Pack<E, V> e = load_pack<E, V>(p + V * lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q.v[i] = elem_to_f32(e.e[i]);
+      for (int i = 0; i < V; ++i) q.v[i] = elem_to_f32(e.e[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q.v[i] = other;
+      for (int i = 0; i < V; ++i) q.v[i] = other;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = lane + 32 * i < n ? elem_to_f32(p[lane + 32 * i]) : other;
+    for (int i = 0; i < V; ++i) q.v[i] = lane + 32 * i < n ? elem_to_f32(p[lane + 32 * i]) : other;
   }
   return q;
 }
 
-template <bool ALIGNED, typename E>
-__device__ __forceinline__ void rec_store(E* p, int lane, int n, const Quad& q) {
+template <int V, bool ALIGNED, typename E>
+__device__ __forceinline__ void rec_store(E* p, int lane, int n, const Cols<V>& q) {
   if (ALIGNED) {
-    if (4 * lane < n) {
-      Pack<E, 4> e;
+    if (V * lane < n) {
+      Pack<E, V> e;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e.e[i] = elem_from_f32<E>(q.v[i]);
-      store_pack<E, 4>(p + 4 * lane, e);
+      for (int i = 0; i < V; ++i) e.e[i] = elem_from_f32<E>(q.v[i]);
+      store_pack<E, V>(p + V * lane, e);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < V; ++i)
       if (lane + 32 * i < n) p[lane + 32 * i] = elem_from_f32<E>(q.v[i]);
   }
 }
 
-__device__ __forceinline__ void st_flag(uint32_t* p, uint32_t v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t ld_flag(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ Quad quad_cg(const float* p) {
-  const float4 f = __ldcg(reinterpret_cast<const float4*>(p));
-  return Quad{{f.x, f.y, f.z, f.w}};
-}
-__device__ __forceinline__ void quad_st(float* p, const Quad& q) {
-  *reinterpret_cast<float4*>(p) = make_float4(q.v[0], q.v[1], q.v[2], q.v[3]);
-}
-
-constexpr uint32_t kRecMap = 1, kRecState = 2;  // flag of a tile: its map, then the state behind it, is published
-
-// The state entering a tile, by one warp: walks back over the tiles at
-// tile - chains, tile - 2 chains, ... (`before` of them) to the nearest
-// published state, or to `first`, the state in front of them all, waiting for
-// the maps of the tiles between; then applies these maps in time order.  Every
-// state is the map of its tile applied to the state before, wherever the walk
-// ended, so the result does not depend on the order in which tiles finished.
-template <typename Form>
-__device__ __forceinline__ Quad rec_look_back(const RecPlan& p, int64_t tile, int before, const Quad& first, int lane) {
-  const uint32_t* flags = p.ticket + 1;
-  int found = before;  // tiles between this one and the state
-  for (int base = 0; base < before; base += 32) {
-    const int k = base + lane;  // lane l looks at the l-th tile back of this round
-    uint32_t f = kRecState;     // in front of the first tile: `first`
-    int nearest;
-    uint64_t t_start = 0;
-    for (int polls = 0;; ++polls) {
-      if (k < before) f = ld_flag(flags + (tile - (int64_t)(k + 1) * p.chains));
-      const uint32_t states = __ballot_sync(0xffffffffu, f == kRecState);
-      const uint32_t open = __ballot_sync(0xffffffffu, f == 0);
-      nearest = states ? __ffs(states) - 1 : 32;
-      const uint32_t needed = nearest >= 32 ? 0xffffffffu : (1u << nearest) - 1u;
-      if ((open & needed) == 0) break;
-      if (polls == 0) t_start = global_ns();
-      const bool late = (polls & 63) == 63 && global_ns() - t_start > kSpinLimitNs;
-      if (__any_sync(0xffffffffu, late)) {  // a predecessor never published: report, and leave with a wrong state
-        if (lane == 0) report_device_error(SPK_DEV_SCAN_TIMEOUT);
-        return first;
-      }
-    }
-    if (nearest < 32) {
-      found = base + nearest;
-      break;
-    }
-  }
-  __syncwarp();
-  Quad s = found < before ? quad_cg(p.states + (tile - (int64_t)(found + 1) * p.chains) * kRecCols + 4 * lane) : first;
-#pragma unroll 4
-  for (int j = found; j > 0; --j) {
-    const float* m = p.maps + (tile - (int64_t)j * p.chains) * 2 * kRecCols + 4 * lane;
-    const Quad A = quad_cg(m), H = quad_cg(m + kRecCols);
+// Maps in shared memory are in the lanes' order: channel i of a lane at V lane + i.
+template <int V>
+__device__ __forceinline__ Cols<V> cols_ld(const float* p, int lane) {
+  const Pack<float, V> e = load_pack<float, V>(p + V * lane);
+  Cols<V> q;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s.v[i] = Form::apply(A.v[i], s.v[i], H.v[i]);
-  }
-  return s;
+  for (int i = 0; i < V; ++i) q.v[i] = e.e[i];
+  return q;
+}
+template <int V>
+__device__ __forceinline__ void cols_st(float* p, int lane, const Cols<V>& q) {
+  Pack<float, V> e;
+#pragma unroll
+  for (int i = 0; i < V; ++i) e.e[i] = q.v[i];
+  store_pack<float, V>(p + V * lane, e);
 }
 
-// Publishes one warp's worth of data (the lanes' quads, already stored) of a tile.
-__device__ __forceinline__ void rec_publish(const RecPlan& p, int64_t tile, uint32_t what, int lane) {
-  __threadfence();
-  __syncwarp();
-  if (lane == 0) st_flag(p.ticket + 1 + tile, what);
+// Where a warp's part of a tile lies: S steps from t0, of which the first
+// `steps` are before the row's end and `room` before the tensor's, n channels
+// from col (all counts 0: nothing there, the state stays).
+struct RecSpot {
+  int64_t b, col, t0;
+  int n, steps, room;
+};
+
+template <int S>
+__device__ __forceinline__ void rec_extent(const RecArgs& a, int cols, RecSpot* q) {
+  q->n = (int)min64(a.D - q->col, cols);
+  q->steps = (int)max64(min64(rec_len(a, q->b) - q->t0, S), 0);
+  q->room = (int)max64(min64(a.L - q->t0, S), 0);
 }
 
-// One warp's part of joining a tile: publishes the tile's map (of the warps'
-// maps sA, sH, in time order or in reverse), looks back, publishes the state
-// behind the tile (unless it is the last of its chain) and returns the one
-// in front of it.
-template <typename Form>
-__device__ __forceinline__ Quad rec_join(const RecPlan& p, int64_t tile, int before, const Quad& first,
-                                         const float (*sA)[kRecCols], const float (*sH)[kRecCols], bool reverse,
-                                         int lane, Quad* behind) {
-  const bool more = before + 1 < p.chunks;
-  Quad A, H;
-  if (more) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      A.v[i] = Form::kept();
-      H.v[i] = 0.0f;
-    }
-#pragma unroll
-    for (int k = 0; k < kRecWarps; ++k) {
-      const int w = reverse ? kRecWarps - 1 - k : k;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        H.v[i] = Form::apply(sA[w][4 * lane + i], H.v[i], sH[w][4 * lane + i]);
-        A.v[i] = Form::join(A.v[i], sA[w][4 * lane + i]);
-      }
-    }
-    if (before > 0) {
-      float* m = p.maps + tile * 2 * kRecCols + 4 * lane;
-      quad_st(m, A);
-      quad_st(m + kRecCols, H);
-      rec_publish(p, tile, kRecMap, lane);
-    }
-  }
-  const Quad s = before > 0 ? rec_look_back<Form>(p, tile, before, first, lane) : first;
-  if (more) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) behind->v[i] = Form::apply(A.v[i], s.v[i], H.v[i]);
-    quad_st(p.states + tile * kRecCols + 4 * lane, *behind);
-    rec_publish(p, tile, kRecState, lane);
-  }
-  return s;
+// An input may be fetched ahead where a lane's piece is what cp.async moves.
+template <typename E, int V, bool ALIGNED>
+__host__ __device__ constexpr bool rec_ahead() {
+  return ALIGNED && V * sizeof(E) >= 4;
 }
 
-// The block's tile: the chunk (time) and chain of this warp; false past the end.
-template <bool SPLIT>
-__device__ __forceinline__ bool rec_tile(const RecPlan& p, int warp, int64_t* tile, int* chunk, int64_t* chain) {
-  if (SPLIT) {
-    __shared__ uint32_t s_ticket;
-    if (threadIdx.x == 0) s_ticket = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-    *tile = s_ticket;
-    *chunk = (int)(*tile / p.chains);
-    *chain = *tile - (int64_t)*chunk * p.chains;
-    return true;
+// The S pieces of one input on their way; a step behind the row's end gets `other`.
+template <typename E, int V, int S>
+__device__ __forceinline__ void rec_copy(E* stage, const void* base, int64_t stride_b, int64_t stride_t,
+                                         const RecSpot& q, int lane, float other) {
+  const E* p = static_cast<const E*>(base) + q.b * stride_b + q.t0 * stride_t + q.col + V * lane;
+  const int steps = V * lane < q.n ? q.steps : 0;
+#pragma unroll
+  for (int j = 0; j < S; ++j) {
+    if (j < steps) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(stage + j * 32 * V)), "l"(p),
+                   "n"(V * sizeof(E) >= 4 ? V * sizeof(E) : 4)
+                   : "memory");
+    } else {
+      Pack<E, V> e;
+#pragma unroll
+      for (int i = 0; i < V; ++i) e.e[i] = elem_from_f32<E>(other);
+      store_pack<E, V>(stage + j * 32 * V, e);
+    }
+    p += stride_t;
   }
-  *tile = blockIdx.x;
-  *chunk = 0;
-  *chain = (int64_t)blockIdx.x * (kRecWarps / p.wt) + warp / p.wt;
-  return *chain < p.chains;
 }
 
-template <typename E, typename Form, bool ALIGNED, bool SPLIT>
-__global__ void __launch_bounds__(32 * kRecWarps, 2) recurrence_kernel(RecArgs a, RecPlan p) {
-  __shared__ float sA[kRecWarps][kRecCols], sH[kRecWarps][kRecCols], sC[kRecCols];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t tile, chain;
-  int chunk;
-  const bool live = rec_tile<SPLIT>(p, warp, &tile, &chunk, &chain);
-  const int wt = SPLIT ? kRecWarps : p.wt, w = SPLIT ? warp : warp % wt;
-  const int64_t b = live ? chain / p.groups : 0, col = live ? (chain - b * p.groups) * kRecCols : 0;
-  const int n = live ? (int)min64(a.D - col, kRecCols) : 0;
-  const int64_t t0 = (int64_t)chunk * kRecChunk + w * kRecSteps;
-  const int64_t len = live ? rec_len(a, b) : 0;
-  const E* x = static_cast<const E*>(a.x) + b * a.x_b + t0 * a.x_t + col;
-  const E* gate = static_cast<const E*>(a.gate) + b * a.g_b + t0 * a.g_t + col;
-  Quad c[kRecSteps], u[kRecSteps];
+template <typename E, int V, int S, bool ALIGNED>
+__device__ __forceinline__ void rec_take(Cols<V>* v, const E* stage, const void* base, int64_t stride_b,
+                                         int64_t stride_t, const RecSpot& q, int lane, float other) {
+  if (rec_ahead<E, V, ALIGNED>()) {
 #pragma unroll
-  for (int j = 0; j < kRecSteps; ++j) {  // a step behind the end keeps the state
-    const int m = t0 + j < len ? n : 0;
-    c[j] = rec_load<ALIGNED>(gate + j * a.g_t, lane, m, Form::kept_gate());
-    u[j] = rec_load<ALIGNED>(x + j * a.x_t, lane, m, 0.0f);
-  }
-  Quad h = {{0.0f, 0.0f, 0.0f, 0.0f}};
-  if (!SPLIT && a.h0 != nullptr) h = rec_load<ALIGNED>(a.h0 + b * a.D + col, lane, n, 0.0f);
+    for (int j = 0; j < S; ++j) {
+      const Pack<E, V> e = load_pack<E, V>(stage + j * 32 * V);
 #pragma unroll
-  for (int j = 0; j < kRecSteps; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[j].v[i] = Form::coeff(c[j].v[i]);
-  if (SPLIT || wt > 1) {
-    Quad A, H;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      A.v[i] = c[0].v[i];
-      H.v[i] = Form::step(0.0f, c[0].v[i], u[0].v[i]);
+      for (int i = 0; i < V; ++i) v[j].v[i] = elem_to_f32(e.e[i]);
     }
+  } else {
+    const E* p = static_cast<const E*>(base) + q.b * stride_b + q.t0 * stride_t + q.col;
 #pragma unroll
-    for (int j = 1; j < kRecSteps; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        H.v[i] = Form::step(H.v[i], c[j].v[i], u[j].v[i]);
-        A.v[i] = Form::join(A.v[i], c[j].v[i]);
-      }
-    quad_st(&sA[warp][4 * lane], A);
-    quad_st(&sH[warp][4 * lane], H);
-    __syncthreads();
-    if (SPLIT) {
-      if (warp == 0) {
-        Quad first = {{0.0f, 0.0f, 0.0f, 0.0f}}, behind;
-        if (a.h0 != nullptr) first = rec_load<ALIGNED>(a.h0 + b * a.D + col, lane, n, 0.0f);
-        quad_st(&sC[4 * lane], rec_join<Form>(p, tile, chunk, first, sA, sH, false, lane, &behind));
-        if (chunk + 1 < p.chunks && a.carry != nullptr)
-          rec_store<ALIGNED>(a.carry + ((int64_t)chunk * a.B + b) * a.D + col, lane, n, behind);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h.v[i] = sC[4 * lane + i];
+    for (int j = 0; j < S; ++j) {
+      v[j] = rec_load<V, ALIGNED>(p, lane, j < q.steps ? q.n : 0, other);
+      p += stride_t;
     }
-    for (int k = warp - w; k < warp; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h.v[i] = Form::apply(sA[k][4 * lane + i], h.v[i], sH[k][4 * lane + i]);
   }
-  if (!live) return;
-  E* out = static_cast<E*>(a.h) + b * a.h_b + t0 * a.h_t + col;
-  const Quad zero = {{0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-  for (int j = 0; j < kRecSteps; ++j) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h.v[i] = Form::step(h.v[i], c[j].v[i], u[j].v[i]);
-    if (t0 + j < a.L) rec_store<ALIGNED>(out + j * a.h_t, lane, n, t0 + j < len ? h : zero);
-  }
-  if (chunk + 1 == p.chunks && w + 1 == wt) rec_store<ALIGNED>(a.last + b * a.D + col, lane, n, h);
 }
 
-// Backward: the same tiles, taken from the end.  A tile runs its steps forward
-// from the state the forward pass kept (h is not read back from memory, where
-// it was rounded), and backwards from the gradient that reaches it, whose
-// affine map has the same decay.
-template <typename E, typename Form, bool ALIGNED, bool SPLIT>
-__global__ void __launch_bounds__(32 * kRecWarps, 2) recurrence_backward_kernel(RecArgs a, RecPlan p) {
-  __shared__ float sA[kRecWarps][kRecCols], sH[kRecWarps][kRecCols], sG[kRecWarps][kRecCols], sC[kRecCols];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t tile, chain;
-  int back;
-  const bool live = rec_tile<SPLIT>(p, warp, &tile, &back, &chain);
-  const int chunk = p.chunks - 1 - back;
-  const int wt = SPLIT ? kRecWarps : p.wt, w = SPLIT ? warp : warp % wt;
-  const int64_t b = live ? chain / p.groups : 0, col = live ? (chain - b * p.groups) * kRecCols : 0;
-  const int n = live ? (int)min64(a.D - col, kRecCols) : 0;
-  const int64_t t0 = (int64_t)chunk * kRecChunk + w * kRecSteps;
-  const int64_t len = live ? rec_len(a, b) : 0;
-  const E* x = static_cast<const E*>(a.x) + b * a.x_b + t0 * a.x_t + col;
-  const E* gate = static_cast<const E*>(a.gate) + b * a.g_b + t0 * a.g_t + col;
-  const E* gh = static_cast<const E*>(a.gh) + b * a.h_b + t0 * a.h_t + col;
-  const Quad zero = {{0.0f, 0.0f, 0.0f, 0.0f}};
-  Quad c[kRecSteps], u[kRecSteps], g[kRecSteps];
-#pragma unroll
-  for (int j = 0; j < kRecSteps; ++j) {
-    const int m = t0 + j < len ? n : 0;
-    c[j] = rec_load<ALIGNED>(gate + j * a.g_t, lane, m, Form::kept_gate());
-    u[j] = rec_load<ALIGNED>(x + j * a.x_t, lane, m, 0.0f);
-    g[j] = rec_load<ALIGNED>(gh + j * a.h_t, lane, a.gh != nullptr ? m : 0, 0.0f);
+template <typename E, int V, int S, bool ALIGNED>
+constexpr size_t rec_stage_bytes(int tensors) {
+  return rec_ahead<E, V, ALIGNED>() ? (size_t)tensors * kRecWarps * S * 32 * V * sizeof(E) : 0;
+}
+
+// A lane's inputs of a forward tile and the places they travel through.
+template <typename E, int V, int S, bool ALIGNED>
+struct RecInputs {
+  E* stage;
+  int lane;
+  static constexpr int kStep = kRecWarps * S * 32 * V;  // between the tensors' stages
+
+  __device__ __forceinline__ RecInputs(unsigned char* smem, int warp, int lane_)
+      : stage(reinterpret_cast<E*>(smem) + warp * S * 32 * V + V * lane_), lane(lane_) {}
+  __device__ __forceinline__ void ask(const RecArgs& a, const RecSpot& q, float kept_gate, bool backward) const {
+    if constexpr (rec_ahead<E, V, ALIGNED>()) {
+      rec_copy<E, V, S>(stage, a.gate, a.g_b, a.g_t, q, lane, kept_gate);
+      rec_copy<E, V, S>(stage + kStep, a.x, a.x_b, a.x_t, q, lane, 0.0f);
+      if (backward && a.gh != nullptr) rec_copy<E, V, S>(stage + 2 * kStep, a.gh, a.h_b, a.h_t, q, lane, 0.0f);
+    }
   }
-  Quad h = zero, later = zero;
-  if (live) {
-    const float* start = chunk > 0 ? a.carry + ((int64_t)(chunk - 1) * a.B + b) * a.D + col
-                                   : (a.h0 != nullptr ? a.h0 + b * a.D + col : nullptr);
-    if (start != nullptr) h = rec_load<ALIGNED>(start, lane, n, 0.0f);
-    if (a.glast != nullptr && (!SPLIT || warp == 0)) later = rec_load<ALIGNED>(a.glast + b * a.D + col, lane, n, 0.0f);
+  __device__ __forceinline__ void wait() const {
+    if constexpr (rec_ahead<E, V, ALIGNED>()) asm volatile("cp.async.wait_all;" ::: "memory");
   }
+  __device__ __forceinline__ void gate(const RecArgs& a, const RecSpot& q, Cols<V>* v, float other) const {
+    rec_take<E, V, S, ALIGNED>(v, stage, a.gate, a.g_b, a.g_t, q, lane, other);
+  }
+  __device__ __forceinline__ void x(const RecArgs& a, const RecSpot& q, Cols<V>* v) const {
+    rec_take<E, V, S, ALIGNED>(v, stage + kStep, a.x, a.x_b, a.x_t, q, lane, 0.0f);
+  }
+  __device__ __forceinline__ void gh(const RecArgs& a, const RecSpot& q, Cols<V>* v) const {
+    if (a.gh != nullptr) {
+      rec_take<E, V, S, ALIGNED>(v, stage + 2 * kStep, a.gh, a.h_b, a.h_t, q, lane, 0.0f);
+    } else {
 #pragma unroll
-  for (int j = 0; j < kRecSteps; ++j)
+      for (int j = 0; j < S; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[j].v[i] = Form::coeff(c[j].v[i]);
-  if (SPLIT || wt > 1) {
-    Quad A, H, G;
+        for (int i = 0; i < V; ++i) v[j].v[i] = 0.0f;
+    }
+  }
+};
+
+template <int V>
+__device__ __forceinline__ Cols<V> cols_of(float f) {
+  Cols<V> q;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      A.v[i] = c[0].v[i];
-      H.v[i] = Form::step(0.0f, c[0].v[i], u[0].v[i]);
-      G.v[i] = 0.0f;
+  for (int i = 0; i < V; ++i) q.v[i] = f;
+  return q;
+}
+
+template <typename Form, int V>
+__device__ __forceinline__ void cols_apply(const float* A, const float* H, int lane, Cols<V>* h) {
+  const Cols<V> pA = cols_ld<V>(A, lane), pH = cols_ld<V>(H, lane);
+#pragma unroll
+  for (int i = 0; i < V; ++i) h->v[i] = Form::apply(pA.v[i], h->v[i], pH.v[i]);
+}
+
+// The gates become decays, and the warp's steps one map (A, H).
+template <typename Form, int V, int S>
+__device__ __forceinline__ void rec_reduce(Cols<V>* c, const Cols<V>* u, Cols<V>* A, Cols<V>* H) {
+  *A = cols_of<V>(Form::open());
+  *H = cols_of<V>(0.0f);
+#pragma unroll
+  for (int j = 0; j < S; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float e;
+      c[j].v[i] = Form::coeff(c[j].v[i], &e);
+      H->v[i] = Form::step(H->v[i], c[j].v[i], u[j].v[i]);
+      A->v[i] = Form::more(A->v[i], c[j].v[i], e);
     }
 #pragma unroll
-    for (int j = 1; j < kRecSteps; ++j)
+  for (int i = 0; i < V; ++i) A->v[i] = Form::close(A->v[i]);
+}
+
+template <typename Form, int V, int S>
+__device__ __forceinline__ void rec_coeffs(Cols<V>* c) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        H.v[i] = Form::step(H.v[i], c[j].v[i], u[j].v[i]);
-        A.v[i] = Form::join(A.v[i], c[j].v[i]);
-      }
+  for (int j = 0; j < S; ++j)
 #pragma unroll
-    for (int j = kRecSteps - 1; j >= 0; --j)
+    for (int i = 0; i < V; ++i) c[j].v[i] = Form::coeff(c[j].v[i]);
+}
+
+// The gradient's map of the warp's steps (its decay is A too).
+template <typename Form, int V, int S>
+__device__ __forceinline__ Cols<V> rec_reduce_back(const Cols<V>* c, const Cols<V>* g) {
+  Cols<V> G = cols_of<V>(0.0f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) G.v[i] = Form::back(g[j].v[i] + G.v[i], c[j].v[i]);
-    quad_st(&sA[warp][4 * lane], A);
-    quad_st(&sH[warp][4 * lane], H);
-    quad_st(&sG[warp][4 * lane], G);
-    __syncthreads();
-    if (SPLIT) {
-      if (warp == 0) {
-        Quad behind;
-        quad_st(&sC[4 * lane], rec_join<Form>(p, tile, back, later, sA, sG, true, lane, &behind));
-      }
-    }
-    for (int k = warp - w; k < warp; ++k)
+  for (int j = S - 1; j >= 0; --j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h.v[i] = Form::apply(sA[k][4 * lane + i], h.v[i], sH[k][4 * lane + i]);
+    for (int i = 0; i < V; ++i) G.v[i] = Form::back(g[j].v[i] + G.v[i], c[j].v[i]);
+  return G;
+}
+
+// The warp's states from h on, written; h becomes the state behind them.
+template <typename E, typename Form, int V, int S, bool ALIGNED>
+__device__ __forceinline__ void rec_run_forward(const RecArgs& a, const RecSpot& q, const Cols<V>* c, const Cols<V>* u,
+                                                Cols<V>* h, int lane) {
+  E* out = static_cast<E*>(a.h) + q.b * a.h_b + q.t0 * a.h_t + q.col;
+#pragma unroll
+  for (int j = 0; j < S; ++j) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) h->v[i] = Form::step(h->v[i], c[j].v[i], u[j].v[i]);
+    if (j < q.room) rec_store<V, ALIGNED>(out, lane, q.n, j < q.steps ? *h : cols_of<V>(0.0f));
+    out += a.h_t;
   }
-  // forward once more; what dgate needs of the state takes x's place
+}
+
+// The warp's states from h on; what dgate needs of them takes x's place.
+template <typename Form, int V, int S>
+__device__ __forceinline__ void rec_replay(const Cols<V>* c, Cols<V>* u, Cols<V> h) {
 #pragma unroll
-  for (int j = 0; j < kRecSteps; ++j)
+  for (int j = 0; j < S; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < V; ++i) {
       const float before = h.v[i];
       h.v[i] = Form::step(before, c[j].v[i], u[j].v[i]);
       u[j].v[i] = Form::grad_base(before, u[j].v[i]);
     }
-  if (SPLIT || wt > 1) {
-    if (SPLIT) {
+}
+
+// The warp's gradients from the one that reaches its last step, written;
+// `later` becomes the one that reaches the step before its first.
+template <typename E, typename Form, int V, int S, bool ALIGNED>
+__device__ __forceinline__ void rec_run_back(const RecArgs& a, const RecSpot& q, const Cols<V>* c, const Cols<V>* u,
+                                             const Cols<V>* g, Cols<V>* later, int lane) {
+  const int64_t end = q.b * a.o_b + (q.t0 + S - 1) * a.o_t + q.col;
+  E *dx = static_cast<E*>(a.dx) + end, *dg = static_cast<E*>(a.dgate) + end;
+#pragma unroll
+  for (int j = S - 1; j >= 0; --j) {
+    Cols<V> ox, og;
+    const bool on = j < q.steps;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float total = g[j].v[i] + later->v[i];
+      ox.v[i] = on ? Form::dx(total, c[j].v[i]) : 0.0f;
+      og.v[i] = on ? Form::dgate(total, c[j].v[i], u[j].v[i]) : 0.0f;
+      later->v[i] = Form::back(total, c[j].v[i]);
+    }
+    if (j < q.room) {
+      rec_store<V, ALIGNED>(dx, lane, q.n, ox);
+      rec_store<V, ALIGNED>(dg, lane, q.n, og);
+    }
+    dx -= a.o_t;
+    dg -= a.o_t;
+  }
+}
+
+// ---- up to 64 steps: `wt` warps of a block along time (the fewest powers of
+// two that hold them), 8 / wt along chains; blocks take every gridDim-th tile.
+template <int S>
+__device__ __forceinline__ RecSpot rec_short_spot(const RecArgs& a, const RecPlan& p, int64_t tile, int warp) {
+  RecSpot q{};
+  const int64_t chain = tile * (kRecWarps / p.wt) + warp / p.wt;
+  if (chain >= p.chains) return q;
+  q.b = chain / p.groups;
+  q.col = (chain - q.b * p.groups) * 128;
+  q.t0 = (warp % p.wt) * S;
+  rec_extent<S>(a, 128, &q);
+  return q;
+}
+
+template <typename E, typename Form, int S, bool ALIGNED>
+__global__ void __launch_bounds__(kRecThreads, 2) recurrence_short_kernel(RecArgs a, RecPlan p) {
+  constexpr int V = 4;
+  extern __shared__ __align__(16) unsigned char rec_smem[];
+  __shared__ __align__(16) float mA[2][kRecWarps][32 * V], mH[2][kRecWarps][32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % p.wt;
+  const RecInputs<E, V, S, ALIGNED> in(rec_smem, warp, lane);
+  RecSpot q = rec_short_spot<S>(a, p, blockIdx.x, warp);
+  in.ask(a, q, Form::kept_gate(), false);
+  int round = 0;
+  for (int64_t tile = blockIdx.x; tile < p.tiles; tile += gridDim.x, round ^= 1) {
+    Cols<V> c[S], u[S];
+    in.wait();
+    in.gate(a, q, c, Form::kept_gate());
+    in.x(a, q, u);
+    const RecSpot next = rec_short_spot<S>(a, p, tile + gridDim.x, warp);
+    in.ask(a, next, Form::kept_gate(), false);
+    Cols<V> h = cols_of<V>(0.0f);
+    if (a.h0 != nullptr) h = rec_load<V, ALIGNED>(a.h0 + q.b * a.D + q.col, lane, q.n, 0.0f);
+    if (p.wt > 1) {
+      Cols<V> A, H;
+      rec_reduce<Form, V, S>(c, u, &A, &H);
+      cols_st<V>(mA[round][warp], lane, A);
+      cols_st<V>(mH[round][warp], lane, H);
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) later.v[i] = sC[4 * lane + i];
+      for (int k = warp - w; k < warp; ++k) cols_apply<Form, V>(mA[round][k], mH[round][k], lane, &h);
+    } else {
+      rec_coeffs<Form, V, S>(c);
     }
-    for (int k = warp - w + wt - 1; k > warp; --k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) later.v[i] = Form::apply(sA[k][4 * lane + i], later.v[i], sG[k][4 * lane + i]);
+    rec_run_forward<E, Form, V, S, ALIGNED>(a, q, c, u, &h, lane);
+    if (w + 1 == p.wt) rec_store<V, ALIGNED>(a.last + q.b * a.D + q.col, lane, q.n, h);
+    q = next;
   }
-  if (!live) return;
-  E* dx = static_cast<E*>(a.dx) + b * a.o_b + t0 * a.o_t + col;
-  E* dg = static_cast<E*>(a.dgate) + b * a.o_b + t0 * a.o_t + col;
-#pragma unroll
-  for (int j = kRecSteps - 1; j >= 0; --j) {
-    Quad ox, og;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float total = g[j].v[i] + later.v[i];
-      ox.v[i] = Form::dx(total, c[j].v[i]);
-      og.v[i] = Form::dgate(total, c[j].v[i], u[j].v[i]);
-      later.v[i] = Form::back(total, c[j].v[i]);
+}
+
+template <typename E, typename Form, int S, bool ALIGNED>
+__global__ void __launch_bounds__(kRecThreads, 2) recurrence_short_backward_kernel(RecArgs a, RecPlan p) {
+  constexpr int V = 4;
+  extern __shared__ __align__(16) unsigned char rec_smem[];
+  __shared__ __align__(16) float mA[kRecWarps][32 * V], mH[kRecWarps][32 * V], mG[kRecWarps][32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % p.wt;
+  const RecInputs<E, V, S, ALIGNED> in(rec_smem, warp, lane);
+  RecSpot q = rec_short_spot<S>(a, p, blockIdx.x, warp);
+  in.ask(a, q, Form::kept_gate(), true);
+  for (int64_t tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+    Cols<V> c[S], u[S], g[S];
+    in.wait();
+    in.gate(a, q, c, Form::kept_gate());
+    in.x(a, q, u);
+    in.gh(a, q, g);
+    const RecSpot next = rec_short_spot<S>(a, p, tile + gridDim.x, warp);
+    in.ask(a, next, Form::kept_gate(), true);
+    Cols<V> h = cols_of<V>(0.0f), later = cols_of<V>(0.0f);
+    if (a.h0 != nullptr) h = rec_load<V, ALIGNED>(a.h0 + q.b * a.D + q.col, lane, q.n, 0.0f);
+    if (a.glast != nullptr) later = rec_load<V, ALIGNED>(a.glast + q.b * a.D + q.col, lane, q.n, 0.0f);
+    if (p.wt > 1) {
+      Cols<V> A, H;
+      rec_reduce<Form, V, S>(c, u, &A, &H);
+      cols_st<V>(mA[warp], lane, A);
+      cols_st<V>(mH[warp], lane, H);
+      cols_st<V>(mG[warp], lane, rec_reduce_back<Form, V, S>(c, g));
+      __syncthreads();
+      for (int k = warp - w; k < warp; ++k) cols_apply<Form, V>(mA[k], mH[k], lane, &h);
+      for (int k = warp - w + p.wt - 1; k > warp; --k) cols_apply<Form, V>(mA[k], mG[k], lane, &later);
+      __syncthreads();  // the maps are read: the next tile's may come
+    } else {
+      rec_coeffs<Form, V, S>(c);
     }
-    if (t0 + j < a.L) {
-      const bool on = t0 + j < len;
-      rec_store<ALIGNED>(dx + j * a.o_t, lane, n, on ? ox : zero);
-      rec_store<ALIGNED>(dg + j * a.o_t, lane, n, on ? og : zero);
-    }
+    rec_replay<Form, V, S>(c, u, h);
+    rec_run_back<E, Form, V, S, ALIGNED>(a, q, c, u, g, &later, lane);
+    if (a.dh0 != nullptr && w == 0) rec_store<V, ALIGNED>(a.dh0 + q.b * a.D + q.col, lane, q.n, later);
+    q = next;
   }
-  if (a.dh0 != nullptr && chunk == 0 && w == 0) rec_store<ALIGNED>(a.dh0 + b * a.D + col, lane, n, later);
+}
+
+// ---- longer sequences: one cluster of K blocks per chain walks along time,
+// K tiles of 8 S steps at once.  The tiles' maps are exchanged through the
+// cluster's shared memory; every block applies all of them in time order, so
+// each knows the state in front of its own tile and the one behind them all,
+// which it carries on: no block waits for another cluster, x and gate are
+// read once however few chains there are, and the order of every sum is fixed.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
+  uint32_t there;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+  return v;
+}
+
+// Thread < 32 V: its channel's part of joining the tiles.  `share` publishes
+// the block's map (of the warps' maps, in time order or in reverse) in
+// `mine`[2][32 V]; after the cluster's barrier, `meet` applies the K maps (in
+// the order of ranks, or in reverse) to `state`, the one in front of them all,
+// returns the one in front of this block's tile and moves `state` behind them.
+template <typename Form, int V>
+__device__ __forceinline__ void rec_share(const float (*mA)[32 * V], const float (*mH)[32 * V], bool reverse,
+                                          float* mine, int c) {
+  float A = Form::kept(), H = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kRecWarps; ++k) {
+    const int w = reverse ? kRecWarps - 1 - k : k;
+    H = Form::apply(mA[w][c], H, mH[w][c]);
+    A = Form::join(A, mA[w][c]);
+  }
+  mine[c] = A;
+  mine[32 * V + c] = H;
+}
+
+template <typename Form, int V>
+__device__ __forceinline__ float rec_meet(const float* mine, bool reverse, int rank, int K, int c, float* state) {
+  const uint32_t at = smem_u32(mine + c);
+  float s = *state, front = s;
+#pragma unroll 4
+  for (int k = 0; k < K; ++k) {
+    const int r = reverse ? K - 1 - k : k;
+    const float A = cluster_load(at, r), H = cluster_load(at + 4 * 32 * V, r);
+    if (r == rank) front = s;
+    s = Form::apply(A, s, H);
+  }
+  *state = s;
+  return front;
+}
+
+template <int V, int S>
+__device__ __forceinline__ RecSpot rec_long_spot(const RecArgs& a, const RecPlan& p, int64_t chain, int64_t chunk,
+                                                 int warp) {
+  RecSpot q{};
+  q.b = chain / p.groups;
+  q.col = (chain - q.b * p.groups) * (32 * V);
+  q.t0 = (chunk * kRecWarps + warp) * S;
+  if (chunk < 0 || chunk >= p.chunks) return q;  // nothing there: the state stays
+  rec_extent<S>(a, 32 * V, &q);
+  return q;
+}
+
+template <typename E, typename Form, int V, int S, bool ALIGNED>
+__global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_kernel(RecArgs a, RecPlan p) {
+  extern __shared__ __align__(16) unsigned char rec_smem[];
+  __shared__ __align__(16) float mA[2][kRecWarps][32 * V], mH[2][kRecWarps][32 * V], mine[2][2 * 32 * V], sC[32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = threadIdx.x;
+  const int rank = (int)cluster_rank(), K = (int)cluster_size();
+  const int64_t chain = blockIdx.x / K;
+  const RecInputs<E, V, S, ALIGNED> in(rec_smem, warp, lane);
+  RecSpot q = rec_long_spot<V, S>(a, p, chain, rank, warp);
+  in.ask(a, q, Form::kept_gate(), false);
+  const int width = (int)min64(a.D - q.col, 32 * V), ch = rec_col<V, ALIGNED>(slot / V, slot % V);
+  const bool joins = slot < 32 * V;  // this thread joins the tiles for channel ch
+  float state = joins && ch < width && a.h0 != nullptr ? a.h0[q.b * a.D + q.col + ch] : 0.0f;
+  int round = 0;
+  for (int64_t first = 0; first < p.chunks; first += K, round ^= 1) {
+    const int64_t chunk = first + rank;
+    Cols<V> c[S], u[S], A, H;
+    in.wait();
+    in.gate(a, q, c, Form::kept_gate());
+    in.x(a, q, u);
+    const RecSpot next = rec_long_spot<V, S>(a, p, chain, chunk + K, warp);
+    in.ask(a, next, Form::kept_gate(), false);
+    rec_reduce<Form, V, S>(c, u, &A, &H);
+    cols_st<V>(mA[round][warp], lane, A);
+    cols_st<V>(mH[round][warp], lane, H);
+    __syncthreads();
+    if (K > 1) {
+      if (joins) rec_share<Form, V>(mA[round], mH[round], false, mine[round], slot);
+      cluster_arrive();
+      cluster_wait();
+    }
+    if (joins) {
+      float front = state;
+      if (K > 1) {
+        front = rec_meet<Form, V>(mine[round], false, rank, K, slot, &state);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kRecWarps; ++k) state = Form::apply(mA[round][k][slot], state, mH[round][k][slot]);
+      }
+      sC[slot] = front;
+      if (a.carry != nullptr && chunk > 0 && chunk < p.chunks && ch < width)
+        a.carry[((chunk - 1) * a.B + q.b) * a.D + q.col + ch] = front;
+    }
+    __syncthreads();
+    Cols<V> h = cols_ld<V>(sC, lane);
+    for (int k = 0; k < warp; ++k) cols_apply<Form, V>(mA[round][k], mH[round][k], lane, &h);
+    rec_run_forward<E, Form, V, S, ALIGNED>(a, q, c, u, &h, lane);
+    q = next;
+  }
+  if (joins && rank == 0 && ch < width) a.last[q.b * a.D + q.col + ch] = state;
+  if (K > 1) {  // the maps of this block may still be read
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
+// Backward: the same tiles from the end.  A tile runs its steps forward from
+// the state the forward pass kept (h is not read back from memory, where it
+// was rounded), and backwards from the gradient that reaches it, whose affine
+// map has the same decay.
+template <typename E, typename Form, int V, int S, bool ALIGNED>
+__global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_backward_kernel(RecArgs a, RecPlan p) {
+  extern __shared__ __align__(16) unsigned char rec_smem[];
+  __shared__ __align__(16) float mA[kRecWarps][32 * V], mH[kRecWarps][32 * V], mG[kRecWarps][32 * V];
+  __shared__ __align__(16) float mine[2][2 * 32 * V], sC[32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = threadIdx.x;
+  const int rank = (int)cluster_rank(), K = (int)cluster_size();
+  const int64_t chain = blockIdx.x / K;
+  const RecInputs<E, V, S, ALIGNED> in(rec_smem, warp, lane);
+  const int64_t top = (p.chunks - 1) / K * K;
+  RecSpot q = rec_long_spot<V, S>(a, p, chain, top + rank, warp);
+  in.ask(a, q, Form::kept_gate(), true);
+  const int width = (int)min64(a.D - q.col, 32 * V), ch = rec_col<V, ALIGNED>(slot / V, slot % V);
+  const bool joins = slot < 32 * V;
+  float state = joins && ch < width && a.glast != nullptr ? a.glast[q.b * a.D + q.col + ch] : 0.0f;
+  int round = 0;
+  for (int64_t first = top; first >= 0; first -= K, round ^= 1) {
+    const int64_t chunk = first + rank;
+    Cols<V> c[S], u[S], g[S], h;
+    in.wait();
+    in.gate(a, q, c, Form::kept_gate());
+    in.x(a, q, u);
+    in.gh(a, q, g);
+    const RecSpot next = rec_long_spot<V, S>(a, p, chain, chunk - K, warp);
+    in.ask(a, next, Form::kept_gate(), true);
+    {
+      Cols<V> A, H;
+      rec_reduce<Form, V, S>(c, u, &A, &H);
+      cols_st<V>(mA[warp], lane, A);
+      cols_st<V>(mH[warp], lane, H);
+      cols_st<V>(mG[warp], lane, rec_reduce_back<Form, V, S>(c, g));
+    }
+    h = cols_of<V>(0.0f);
+    const float* start = chunk > 0 ? a.carry + ((chunk - 1) * a.B + q.b) * a.D : a.h0 + q.b * a.D;
+    if (chunk > 0 || a.h0 != nullptr) h = rec_load<V, ALIGNED>(start + q.col, lane, q.n, 0.0f);
+    __syncthreads();
+    if (K > 1) {
+      if (joins) rec_share<Form, V>(mA, mG, true, mine[round], slot);
+      cluster_arrive();
+    }
+    for (int k = 0; k < warp; ++k) cols_apply<Form, V>(mA[k], mH[k], lane, &h);
+    rec_replay<Form, V, S>(c, u, h);
+    if (K > 1) cluster_wait();
+    if (joins) {
+      float front = state;
+      if (K > 1) {
+        front = rec_meet<Form, V>(mine[round], true, rank, K, slot, &state);
+      } else {
+#pragma unroll
+        for (int k = kRecWarps - 1; k >= 0; --k) state = Form::apply(mA[k][slot], state, mG[k][slot]);
+      }
+      sC[slot] = front;
+    }
+    __syncthreads();
+    Cols<V> later = cols_ld<V>(sC, lane);
+    for (int k = kRecWarps - 1; k > warp; --k) cols_apply<Form, V>(mA[k], mG[k], lane, &later);
+    __syncthreads();  // the maps are read: the next tile's may come
+    rec_run_back<E, Form, V, S, ALIGNED>(a, q, c, u, g, &later, lane);
+    q = next;
+  }
+  if (joins && rank == 0 && ch < width && a.dh0 != nullptr) a.dh0[q.b * a.D + q.col + ch] = state;
+  if (K > 1) {  // the maps of this block may still be read
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 // One step of the recurrence over n cells: out (element type) and the new
@@ -495,17 +729,12 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(const E* __restric
   new_state[i] = h;
 }
 
-template <typename F>
-inline bool with_form(int form, F&& f) {
-  if (form == SPK_REC_GATE) {
+template <typename E, typename F>
+inline void with_form(int form, F&& f) {
+  if (form == SPK_REC_GATE)
     f(GateForm{});
-    return true;
-  }
-  if (form == SPK_REC_LEAKY) {
-    f(LeakyForm{});
-    return true;
-  }
-  return false;
+  else
+    f(LeakyForm<sizeof(E) == 4>{});
 }
 
 // Shape, type and alignment checks shared by the recurrence's entry points.
@@ -517,8 +746,8 @@ static int rec_check(int dtype, int form, int64_t B, int64_t L, int64_t D, size_
   SPK_REQUIRE(form == SPK_REC_GATE || form == SPK_REC_LEAKY, "unknown recurrence form %d", form);
   SPK_REQUIRE(L < (1ll << 31) && D < (1ll << 31) && (D == 0 || B < (1ll << 37) / D),
               "shape too large (B=%lld, L=%lld, D=%lld)", (long long)B, (long long)L, (long long)D);
-  SPK_REQUIRE((double)B * ceil_div(D, kRecCols) * max64(ceil_div(L, kRecChunk), 1) < 2147483647.0,
-              "too many steps and channels (B=%lld, L=%lld, D=%lld)", (long long)B, (long long)L, (long long)D);
+  SPK_REQUIRE(B < (1ll << 31) / (kRecMaxCluster * max64(ceil_div(D, 32), 1)),
+              "too many rows (B=%lld, D=%lld)", (long long)B, (long long)D);
   return SPK_OK;
 }
 
@@ -526,72 +755,143 @@ static bool rec_aligned(const void* p, size_t eb, int64_t stride_b, int64_t stri
   return aligned_to(p, 4 * eb) && stride_b % 4 == 0 && stride_t % 4 == 0;
 }
 
-// Fills the plan from the workspace; batch rows that follow one another like
-// channels (no lengths, batch stride D everywhere) become channels first, so
-// that narrow rows share a warp.
-static void rec_plan(RecArgs* a, RecPlan* p, bool merge, void* workspace) {
+// Channels per chain of a long recurrence: 128 (tiles of 64 steps), or 32
+// (tiles of 256) when clusters of 128-channel chains would leave most of the
+// GPU idle.
+static int rec_long_cols(int64_t B, int64_t D) {
+  return B * ceil_div(D, 128) * kRecMaxCluster >= 128 ? 128 : 32;
+}
+
+static int64_t rec_chunk(int64_t B, int64_t L, int64_t D) {
+  return L <= 64 ? 64 : 64 * (128 / rec_long_cols(B, D));
+}
+
+// Batch rows that follow one another like channels (no lengths, batch stride D
+// everywhere) become channels first, so that narrow rows share a warp.
+static RecPlan rec_plan(RecArgs* a, bool merge) {
+  RecPlan p{};
+  const int64_t chunk = rec_chunk(a->B, a->L, a->D);
+  p.cols = a->L <= 64 ? 128 : rec_long_cols(a->B, a->D);
   if (merge && a->lengths == nullptr) {
     a->D *= a->B;
     a->B = 1;
   }
-  p->groups = ceil_div(a->D, kRecCols);
-  p->chains = a->B * p->groups;
-  p->chunks = (int)max64(ceil_div(a->L, kRecChunk), 1);
-  p->wt = 1;
-  while (p->wt < kRecWarps && (int64_t)p->wt * kRecSteps < a->L) p->wt *= 2;
-  p->tiles = p->chunks > 1 ? p->chains * p->chunks : ceil_div(p->chains, kRecWarps / p->wt);
-  if (p->chunks > 1) {
-    p->ticket = static_cast<uint32_t*>(workspace);
-    p->maps = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(4 * (size_t)(p->tiles + 1), 256));
-    p->states = p->maps + p->tiles * 2 * kRecCols;
-  }
+  p.groups = ceil_div(a->D, p.cols);
+  p.chains = a->B * p.groups;
+  p.chunks = max64(ceil_div(a->L, chunk), 1);
+  p.wt = 1;
+  while (p.wt < kRecWarps && (int64_t)p.wt * 8 < a->L) p.wt *= 2;
+  p.tiles = ceil_div(p.chains, kRecWarps / p.wt);
+  return p;
 }
 
-static int rec_workspace_check(int64_t B, int64_t L, int64_t D, const void* workspace, size_t bytes) {
-  const size_t need = spk_recurrence_workspace_bytes(B, L, D);
-  if (need > 0 && (workspace == nullptr || bytes < need))
-    return fail(SPK_EWORKSPACE, "the recurrence needs a workspace of %zu bytes", need);
-  SPK_REQUIRE(aligned_to(workspace, 16), "the workspace must be 16-byte aligned");
+template <typename E, typename Form, int S, bool ALIGNED>
+static cudaError_t rec_launch_short(bool backward, const RecArgs& a, const RecPlan& p, cudaStream_t st) {
+  auto* const kernel =
+      backward ? recurrence_short_backward_kernel<E, Form, S, ALIGNED> : recurrence_short_kernel<E, Form, S, ALIGNED>;
+  const size_t smem = rec_stage_bytes<E, 4, S, ALIGNED>(backward ? 3 : 2);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<(unsigned)min64(p.tiles, 2 * (int64_t)sm_count()), kRecThreads, smem, st>>>(a, p);
+  return cudaGetLastError();
+}
+
+// Clusters of k blocks of a kernel that run at once, k = 1 .. 16 (0: none).
+struct RecOccupancy {
+  int clusters[kRecMaxCluster + 1];
+};
+
+template <typename K>
+static cudaError_t rec_occupancy(K* kernel, size_t smem, RecOccupancy* out) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  for (int k = 1; k <= kRecMaxCluster && e == cudaSuccess; ++k) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)k);
+    cfg.blockDim = dim3(kRecThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)k;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    out->clusters[k] = 0;
+    if (cudaOccupancyMaxActiveClusters(&out->clusters[k], kernel, &cfg) != cudaSuccess) {
+      out->clusters[k] = 0;
+      (void)cudaGetLastError();
+    }
+  }
+  return e;
+}
+
+template <typename E, typename Form, int V, int S, bool ALIGNED, bool BACKWARD>
+static cudaError_t rec_launch_long(const RecArgs& a, const RecPlan& p, cudaStream_t st) {
+  auto* const kernel = BACKWARD ? recurrence_long_backward_kernel<E, Form, V, S, ALIGNED>
+                                : recurrence_long_kernel<E, Form, V, S, ALIGNED>;
+  const size_t smem = rec_stage_bytes<E, V, S, ALIGNED>(BACKWARD ? 3 : 2);
+  static PerDevice<RecOccupancy> cache;  // one per kernel
+  RecOccupancy occ;
+  cudaError_t e = cache.get(&occ, [&](RecOccupancy* o) { return rec_occupancy(kernel, smem, o); });
+  if (e != cudaSuccess) return e;
+  // The fewest blocks per chain that need the fewest rounds: every cluster
+  // takes ceil(chunks / k) rounds, as many clusters at once as fit.
+  int cluster = 1;
+  int64_t best = 0;
+  for (int k = 1; k <= kRecMaxCluster && k <= p.chunks; ++k) {
+    if (occ.clusters[k] <= 0) continue;
+    const int64_t rounds = ceil_div(p.chains, occ.clusters[k]) * ceil_div(p.chunks, k);
+    if (best == 0 || rounds < best) {
+      best = rounds;
+      cluster = k;
+    }
+  }
+  return launch_dependent_cluster(kernel, dim3((unsigned)(p.chains * cluster)), dim3(kRecThreads), smem, st,
+                                  (unsigned)cluster, false, a, p);
+}
+
+template <typename E, typename Form, int V, int S, bool ALIGNED>
+static cudaError_t rec_launch_long(bool backward, const RecArgs& a, const RecPlan& p, cudaStream_t st) {
+  return backward ? rec_launch_long<E, Form, V, S, ALIGNED, true>(a, p, st)
+                  : rec_launch_long<E, Form, V, S, ALIGNED, false>(a, p, st);
+}
+
+static int rec_run(bool backward, int dtype, int form, bool aligned, const RecArgs& a, const RecPlan& p,
+                   cudaStream_t st) {
+  cudaError_t rc = cudaSuccess;
+  with_elem(dtype, [&](auto e) {
+    using E = decltype(e);
+    with_form<E>(form, [&](auto f) {
+      using F = decltype(f);
+      if (a.L > 64 && p.cols == 32)
+        rc = rec_launch_long<E, F, 1, 32, true>(backward, a, p, st);
+      else if (a.L > 64)
+        rc = aligned ? rec_launch_long<E, F, 4, 8, true>(backward, a, p, st)
+                     : rec_launch_long<E, F, 4, 8, false>(backward, a, p, st);
+      else if (a.L > 4)
+        rc = aligned ? rec_launch_short<E, F, 8, true>(backward, a, p, st)
+                     : rec_launch_short<E, F, 8, false>(backward, a, p, st);
+      else
+        rc = aligned ? rec_launch_short<E, F, 4, true>(backward, a, p, st)
+                     : rec_launch_short<E, F, 4, false>(backward, a, p, st);
+    });
+  });
+  if (rc != cudaSuccess) return fail(SPK_ECUDA, "recurrence launch failed: %s", cudaGetErrorString(rc));
+  count_launch(1);
   return SPK_OK;
 }
 
-// The kernel of a plan, its counters cleared first when tiles are joined.
-#define SPK_REC_LAUNCH(KERNEL)                                                                              \
-  if (p.chunks > 1)                                                                                         \
-    SPK_CUDA_TRY(cudaMemsetAsync(p.ticket, 0, 4 * (size_t)(p.tiles + 1), st));                              \
-  spk::with_elem(dtype, [&](auto e) {                                                                       \
-    spk::with_form(form, [&](auto f) {                                                                      \
-      using E = decltype(e);                                                                                \
-      using F = decltype(f);                                                                                \
-      const dim3 grid((unsigned)p.tiles), block(32 * spk::kRecWarps);                                       \
-      if (p.chunks > 1 && aligned)                                                                          \
-        spk::KERNEL<E, F, true, true><<<grid, block, 0, st>>>(a, p);                                        \
-      else if (p.chunks > 1)                                                                                \
-        spk::KERNEL<E, F, false, true><<<grid, block, 0, st>>>(a, p);                                       \
-      else if (aligned)                                                                                     \
-        spk::KERNEL<E, F, true, false><<<grid, block, 0, st>>>(a, p);                                       \
-      else                                                                                                  \
-        spk::KERNEL<E, F, false, false><<<grid, block, 0, st>>>(a, p);                                      \
-    });                                                                                                     \
-  });                                                                                                       \
-  SPK_LAUNCH_CHECK();                                                                                       \
-  spk::count_launch(1)
-
 }  // namespace spk
 
-extern "C" int spk_recurrence_chunk(void) { return spk::kRecChunk; }
-
-extern "C" size_t spk_recurrence_workspace_bytes(int64_t B, int64_t L, int64_t D) {
-  if (B <= 0 || D <= 0 || L <= spk::kRecChunk) return 0;
-  const size_t tiles = (size_t)(B * spk::ceil_div(D, spk::kRecCols) * spk::ceil_div(L, spk::kRecChunk));
-  return spk::align_up(4 * (tiles + 1), 256) + tiles * 3 * spk::kRecCols * sizeof(float);
+extern "C" int64_t spk_recurrence_chunk(int64_t B, int64_t L, int64_t D) {
+  return B > 0 && L > 0 && D > 0 ? spk::rec_chunk(B, L, D) : 64;
 }
 
 extern "C" int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate,
                               int64_t g_stride_b, int64_t g_stride_t, int dtype, int form, int64_t B, int64_t L,
                               int64_t D, const float* state, const int32_t* lengths, void* h, int64_t h_stride_b,
-                              int64_t h_stride_t, float* last, float* carry, void* workspace, size_t workspace_bytes,
-                              spk_stream_t stream) {
+                              int64_t h_stride_t, float* last, float* carry, spk_stream_t stream) {
   size_t eb = 0;
   if (int rc = spk::rec_check(dtype, form, B, L, D, &eb)) return rc;
   if (B == 0 || D == 0) return SPK_OK;
@@ -601,7 +901,6 @@ extern "C" int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_strid
                   spk::aligned_to(state, 4) && spk::aligned_to(lengths, 4) && spk::aligned_to(last, 4) &&
                   spk::aligned_to(carry, 4),
               "tensors must be aligned to their elements");
-  if (int rc = spk::rec_workspace_check(B, L, D, workspace, workspace_bytes)) return rc;
   spk::RecArgs a{};
   a.x = x;
   a.gate = gate;
@@ -624,10 +923,8 @@ extern "C" int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_strid
                        spk::rec_aligned(h, eb, h_stride_b, h_stride_t) && spk::aligned_to(state, 16) &&
                        spk::aligned_to(last, 16) && spk::aligned_to(carry, 16);
   cudaStream_t st = (cudaStream_t)stream;
-  spk::RecPlan p{};
-  spk::rec_plan(&a, &p, x_stride_b == D && g_stride_b == D && h_stride_b == D, workspace);
-  SPK_REC_LAUNCH(recurrence_kernel);
-  return SPK_OK;
+  const spk::RecPlan p = spk::rec_plan(&a, x_stride_b == D && g_stride_b == D && h_stride_b == D);
+  return spk::rec_run(false, dtype, form, aligned, a, p, st);
 }
 
 extern "C" int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate,
@@ -635,21 +932,19 @@ extern "C" int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_
                                        int64_t gh_stride_t, int dtype, int form, int64_t B, int64_t L, int64_t D,
                                        const float* state, const int32_t* lengths, const float* carry,
                                        const float* glast, void* dx, void* dgate, int64_t d_stride_b,
-                                       int64_t d_stride_t, float* dstate, void* workspace, size_t workspace_bytes,
-                                       spk_stream_t stream) {
+                                       int64_t d_stride_t, float* dstate, spk_stream_t stream) {
   size_t eb = 0;
   if (int rc = spk::rec_check(dtype, form, B, L, D, &eb)) return rc;
   if (B == 0 || D == 0) return SPK_OK;
   SPK_REQUIRE(L == 0 || (x != nullptr && gate != nullptr && dx != nullptr && dgate != nullptr),
               "x, gate, dx and dgate must be non-null");
-  SPK_REQUIRE(L <= spk::kRecChunk || carry != nullptr, "the forward pass's carry is needed above %d steps",
-              spk::kRecChunk);
+  SPK_REQUIRE(L <= spk::rec_chunk(B, L, D) || carry != nullptr, "the forward pass's carry is needed above %lld steps",
+              (long long)spk::rec_chunk(B, L, D));
   SPK_REQUIRE(spk::aligned_to(x, eb) && spk::aligned_to(gate, eb) && spk::aligned_to(gh, eb) &&
                   spk::aligned_to(dx, eb) && spk::aligned_to(dgate, eb) && spk::aligned_to(state, 4) &&
                   spk::aligned_to(lengths, 4) && spk::aligned_to(carry, 4) && spk::aligned_to(glast, 4) &&
                   spk::aligned_to(dstate, 4),
               "tensors must be aligned to their elements");
-  if (int rc = spk::rec_workspace_check(B, L, D, workspace, workspace_bytes)) return rc;
   spk::RecArgs a{};
   a.x = x;
   a.gate = gate;
@@ -679,12 +974,9 @@ extern "C" int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_
                        spk::rec_aligned(dgate, eb, d_stride_b, d_stride_t) && spk::aligned_to(state, 16) &&
                        spk::aligned_to(glast, 16) && spk::aligned_to(carry, 16) && spk::aligned_to(dstate, 16);
   cudaStream_t st = (cudaStream_t)stream;
-  spk::RecPlan p{};
-  spk::rec_plan(&a, &p,
-                x_stride_b == D && g_stride_b == D && d_stride_b == D && (gh == nullptr || gh_stride_b == D),
-                workspace);
-  SPK_REC_LAUNCH(recurrence_backward_kernel);
-  return SPK_OK;
+  const spk::RecPlan p = spk::rec_plan(
+      &a, x_stride_b == D && g_stride_b == D && d_stride_b == D && (gh == nullptr || gh_stride_b == D));
+  return spk::rec_run(true, dtype, form, aligned, a, p, st);
 }
 
 extern "C" int spk_recurrence_step(const void* x, const void* gate, int dtype, int form, int64_t n,
@@ -700,7 +992,7 @@ extern "C" int spk_recurrence_step(const void* x, const void* gate, int dtype, i
   const unsigned blocks = (unsigned)spk::ceil_div(n, 256);
   spk::with_elem(dtype, [&](auto e) {
     using E = decltype(e);
-    spk::with_form(form, [&](auto f) {
+    spk::with_form<E>(form, [&](auto f) {
       spk::recurrence_step_kernel<E, decltype(f)><<<blocks, 256, 0, (cudaStream_t)stream>>>(
           static_cast<const E*>(x), static_cast<const E*>(gate), state, n, static_cast<E*>(out), new_state);
     });

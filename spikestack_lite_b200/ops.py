@@ -665,13 +665,13 @@ def _recurrence_forward(x, gate, state, form, dim, lengths, keep):
     B = x.numel() // (L * D) if x.numel() else (state.numel() // D if D else 0)
     (x, (xb, xt)), (gate, (gb, gt)), (h, (hb, ht)) = _time_major(x, dim), _time_major(gate, dim), _empty_time(x, dim)
     last = torch.empty_like(state)
-    chunk = int(lib.spk_recurrence_chunk())
     carry = None
-    if keep and L > chunk:
-        carry = torch.empty((L + chunk - 1) // chunk - 1, B, D, dtype=torch.float32, device=x.device)
-    ws = _scratch(x, lib.spk_recurrence_workspace_bytes(B, L, D))
+    if keep:
+        chunk = int(lib.spk_recurrence_chunk(B, L, D))
+        if L > chunk:
+            carry = torch.empty((L + chunk - 1) // chunk - 1, B, D, dtype=torch.float32, device=x.device)
     _call(x, "spk_recurrence", ptr(x), xb, xt, ptr(gate), gb, gt, _DTYPES[x.dtype], form, B, L, D, ptr(state),
-          ptr(lengths), ptr(h), hb, ht, ptr(last), ptr(carry), ptr(ws), 0 if ws is None else ws.numel())
+          ptr(lengths), ptr(h), hb, ht, ptr(last), ptr(carry))
     return h, last, carry
 
 
@@ -690,7 +690,7 @@ class _GatedRecurrence(torch.autograd.Function):
         x, gate, state, lengths, carry = ctx.saved_tensors
         if gh is None and glast is None:
             return (None,) * 6
-        dim, lib = ctx.dim, _lib.load()
+        dim = ctx.dim
         L, D = x.shape[dim], x.shape[-1]
         B = state.numel() // D if D else 0
         (x, (xb, xt)), (gate, (gb, gt)) = _time_major(x, dim), _time_major(gate, dim)
@@ -701,10 +701,9 @@ class _GatedRecurrence(torch.autograd.Function):
         dx, (db, dt) = _empty_time(x, dim)
         dgate, _ = _empty_time(x, dim)
         dstate = torch.empty_like(state)
-        ws = _scratch(x, lib.spk_recurrence_workspace_bytes(B, L, D))
         _call(x, "spk_recurrence_backward", ptr(x), xb, xt, ptr(gate), gb, gt, ptr(gh), ghb, ght, _DTYPES[x.dtype],
               ctx.form, B, L, D, ptr(state), ptr(lengths), ptr(carry), ptr(glast), ptr(dx), ptr(dgate), db, dt,
-              ptr(dstate), ptr(ws), 0 if ws is None else ws.numel())
+              ptr(dstate))
         return dx, dgate, dstate, None, None, None
 
 

@@ -199,6 +199,24 @@ def test_empty_and_non_finite():
     assert not h[0, 100:, 2].isfinite().any() and not h[0, 150:, 5].isfinite().any()
 
 
+@pytest.mark.parametrize("form", ["leaky", "gate"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("L", [3, 40, 300])
+def test_non_finite_gates(L, dtype, form):
+    x, gate, state, _, _ = make(2, L, 8, form, DT[dtype], seed=L)
+    clean = ops.gated_recurrence(x.cuda(), gate.cuda(), state.cuda(), form=form)[0]
+    gate[0, L // 2, 2] = float("nan")
+    h, last = ops.gated_recurrence(x.cuda(), gate.cuda(), state.cuda(), form=form)
+    assert h[0, L // 2:, 2].isnan().all() and last[0, 2].isnan()
+    h[0, L // 2:, 2] = clean[0, L // 2:, 2]
+    assert torch.equal(h, clean)
+    if form == "leaky":  # gates without bound: the input itself, or the state kept
+        gate[0, L // 2, 2], gate[1, 0, 3] = -float("inf"), float("inf")
+        h, _ = ops.gated_recurrence(x.cuda(), gate.cuda(), state.cuda())
+        assert h.isfinite().all()
+        assert h[0, L // 2, 2] == x[0, L // 2, 2] and h[1, 0, 3] == state[1, 3].to(DT[dtype])
+
+
 def test_runs_on_a_side_stream_and_in_a_graph():
     x, gate, state, gh, glast = make(2, 300, 64, "leaky", torch.float32, seed=1)
     x, gate, state, gh, glast = (t.cuda() for t in (x, gate, state, gh, glast))

@@ -75,7 +75,7 @@ def test_recurrence_entry_points_reject_bad_arguments(lib):
 
     def fwd(x=P, gate=P, dtype=0, form=1, B=2, L=4, D=8, state=None, lengths=None, h=P, last=P, carry=None):
         return lib.spk_recurrence(x, 32, 8, gate, 32, 8, dtype, form, B, L, D, state, lengths, h, 32, 8, last, carry,
-                                  None, 0, None)
+                                  None)
 
     assert fwd(B=0) == SPK_OK and fwd(D=0) == SPK_OK  # nothing to do
     for bad in (dict(dtype=3), dict(dtype=-1), dict(form=2), dict(B=-1), dict(L=-1), dict(D=-1), dict(x=None),
@@ -86,11 +86,11 @@ def test_recurrence_entry_points_reject_bad_arguments(lib):
 
     def bwd(x=P, gate=P, gh=None, dtype=0, form=1, B=2, L=4, D=8, carry=None, dx=P, dgate=P, glast=None):
         return lib.spk_recurrence_backward(x, 32, 8, gate, 32, 8, gh, 32, 8, dtype, form, B, L, D, None, None, carry,
-                                           glast, dx, dgate, 32, 8, None, None, 0, None)
+                                           glast, dx, dgate, 32, 8, None, None)
 
     assert bwd(B=0) == SPK_OK
     for bad in (dict(dtype=3), dict(form=-1), dict(dx=None), dict(dgate=None), dict(x=None), dict(gh=ODD),
-                dict(glast=ODD), dict(L=lib.spk_recurrence_chunk() + 1)):
+                dict(glast=ODD), dict(L=lib.spk_recurrence_chunk(2, 1 << 20, 8) + 1)):
         assert bwd(**bad) == SPK_EINVAL, bad
     assert b"carry" in lib.spk_last_error()
 
