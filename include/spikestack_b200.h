@@ -330,12 +330,12 @@ int spk_temporal_mean(const float* x, int T, int64_t B, int N, int d, float* mea
  * inputs at t >= len_b are not read, and h is 0 there.  A NaN, or an
  * infinite x, makes the channel's later states non-finite.
  * carry (optional, for the backward pass): fp32
- * [ceil(L / C) - 1, B, D] with C = spk_recurrence_chunk(B, L, D), the states
+ * [ceil(L / C) - 1, B, D] with C = spk_recurrence_chunk(dtype, B, L, D), the states
  * before each chunk of C steps but the first.  Arithmetic is fp32, h rounded once.  No reference
  * counterpart (its GSMC loop, nn/gsmc.py:119-142, is nonlinear in the state
  * and runs step by step). */
 enum { SPK_REC_GATE = 0, SPK_REC_LEAKY = 1 };
-int64_t spk_recurrence_chunk(int64_t B, int64_t L, int64_t D);
+int64_t spk_recurrence_chunk(int dtype, int64_t B, int64_t L, int64_t D);
 int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate, int64_t g_stride_b,
                    int64_t g_stride_t, int dtype, int form, int64_t B, int64_t L, int64_t D, const float* state,
                    const int32_t* lengths, void* h, int64_t h_stride_b, int64_t h_stride_t, float* last,

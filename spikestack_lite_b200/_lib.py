@@ -61,7 +61,7 @@ SIGNATURES = {
     "spk_selftest_wait_timeout": (_I, [_P]),
     "spk_spire_planes": (_I, [_P, _P, _P, _P, _I, _L, _I, _I, _P, _P]),
     "spk_temporal_mean": (_I, [_P, _I, _L, _I, _I, _P, _P, _P]),
-    "spk_recurrence_chunk": (_L, [_L, _L, _L]),
+    "spk_recurrence_chunk": (_L, [_I, _L, _L, _L]),
     "spk_recurrence": (_I, [_P, _L, _L, _P, _L, _L, _I, _I, _L, _L, _L, _P, _P, _P, _L, _L, _P, _P, _P]),
     "spk_recurrence_backward": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P,
                                      _L, _L, _P, _P]),

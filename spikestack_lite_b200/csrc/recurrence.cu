@@ -33,29 +33,66 @@ struct RecArgs {
 struct RecPlan {
   int64_t chains, groups;  // chains = B * groups of neighbouring channels
   int64_t tiles, chunks;   // blocks' tiles (short), tiles along time (long)
-  int wt, cols;            // warps along time (short); channels per chain
+  int wt, cols, cluster;   // warps along time (short); channels per chain; blocks per chain (long)
 };
+
+// Two neighbouring channels: sm_100 multiplies and adds fp32 numbers in pairs.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 two(float f) { return F2{f, f}; }
+__device__ __forceinline__ uint64_t f2_bits(F2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ F2 f2_of(uint64_t r) {
+  F2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, two(-1.0f), a); }
 
 // The decay of one or more steps as one float per form: `coeff` from the gate,
 // `step` the new state, `apply` A h + H for a joined decay A, `join` the decay
-// of two in a row, `back` the gradient that passes a step, dx and dgate the
-// gradients of its inputs (dgate from grad_base of the state before and x).
+// of two in a row, `back` the gradient that passes a step, `grads` that and
+// the gradients of the step's inputs (from `base` of the state before and x).
 // A warp's steps are joined by `open`, one `more` per step and `close`.
 // kept_gate is the gate, kept the decay, of a step that keeps the state.
 struct GateForm {
   __device__ static float kept_gate() { return 1.0f; }
   __device__ static float kept() { return 1.0f; }
   __device__ static float open() { return 1.0f; }
-  __device__ static float coeff(float gate, float* = nullptr) { return gate; }
-  __device__ static float more(float acc, float a, float) { return acc * a; }
+  __device__ static float coeff(float gate) { return gate; }
+  __device__ static F2 coeff(F2 gate, F2*) { return gate; }
+  __device__ static F2 more(F2 acc, F2 a, F2) { return mul2(acc, a); }
   __device__ static float close(float acc) { return acc; }
-  __device__ static float step(float h, float a, float x) { return fmaf(a, h, x); }
   __device__ static float apply(float a, float h, float H) { return fmaf(a, h, H); }
   __device__ static float join(float a, float b) { return a * b; }
-  __device__ static float back(float g, float a) { return a * g; }
-  __device__ static float dx(float g, float) { return g; }
-  __device__ static float grad_base(float h, float) { return h; }
-  __device__ static float dgate(float g, float, float base) { return g * base; }
+  __device__ static float step(float h, float a, float x) { return fmaf(a, h, x); }
+  __device__ static F2 step(F2 h, F2 a, F2 x) { return fma2(a, h, x); }
+  __device__ static F2 back(F2 g, F2 a) { return mul2(a, g); }
+  __device__ static F2 base(F2 h, F2) { return h; }
+  __device__ static F2 grads(F2 g, F2 a, F2 base, F2* dx, F2* dgate) {
+    *dx = g;
+    *dgate = mul2(g, base);
+    return mul2(a, g);
+  }
 };
 
 __device__ __forceinline__ float ex2_fast(float x) {
@@ -63,30 +100,18 @@ __device__ __forceinline__ float ex2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float min_nan(float x, float y) {  // NaN when either is
-  float z;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
-  return z;
-}
-__device__ __forceinline__ float rcp_fast(float x) {  // of a normal number with a normal reciprocal
+__device__ __forceinline__ float rcp_fast(float x) {  // a subnormal result becomes 0
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Leaky form.  Joined decays are whichever of A and Q = 1 - A is at most one
-// half, the sign bit set when it is A: neither a slow channel's Q nor a fast
-// channel's A is a difference from 1.  Over a warp's steps, with e =
-// exp(-gate) and a = 1 / (1 + e), the product of decays is 1 / (1 + E) with
-// E = prod (1 + e) - 1, a sum of positive terms (kept finite: below 2^-124 a
-// joined decay is as good as 0).
-// The decay of one step is kept the same way for fp32 tensors (FINE).  For
-// 16-bit ones it is q itself, and exp is the hardware's: a fast channel's
-// result is then off by a rounding of the state before it and the weights by
-// some 2^-21, far below the 2^-9 or 2^-12 that its inputs and outputs carry,
-// for 16 instead of 33 instructions per element (the 16-bit kernels are
-// bound by instruction issue, the fp32 ones by memory).
-template <bool FINE>
+// Leaky form, fp32 tensors.  A decay, of one step or of several, is whichever
+// of A and Q = 1 - A is at most one half, the sign bit set when it is A:
+// neither a slow channel's Q nor a fast channel's A is a difference from 1.
+// Over a warp's steps, with e = exp(-gate) and a = 1 / (1 + e), the product of
+// decays is 1 / (1 + E) with E = prod (1 + e) - 1, a sum of positive terms
+// (kept finite: below 2^-124 a joined decay is as good as 0).
 struct LeakyForm {
   __device__ static float kept_gate() { return __int_as_float(0x7f800000); }  // q = 0
   __device__ static float kept() { return 0.0f; }
@@ -94,16 +119,17 @@ struct LeakyForm {
   __device__ static bool is_a(float c) { return __float_as_int(c) < 0; }
   // the decay of a step; *e (when wanted) becomes exp(-gate)
   __device__ static float coeff(float gate, float* e = nullptr) {
-    if (!FINE) {
-      const float ex = ex2_fast(min_nan(gate * -1.4426950409f, 124.0f));
-      if (e != nullptr) *e = ex;
-      return ex * rcp_fast(1.0f + ex);
-    }
     const float small = expf(-fabsf(gate));
     if (e != nullptr) *e = gate < 0.0f ? rcp_fast(fmaxf(small, 0x1p-124f)) : small;
     return copysignf(small * rcp_fast(1.0f + small), gate);
   }
-  __device__ static float more(float acc, float, float e) { return fminf(fmaf(acc, e, acc + e), 0x1p124f); }
+  __device__ static F2 coeff(F2 gate, F2* e) {
+    return e != nullptr ? F2{coeff(gate.x, &e->x), coeff(gate.y, &e->y)} : F2{coeff(gate.x), coeff(gate.y)};
+  }
+  __device__ static F2 more(F2 acc, F2, F2 e) {
+    const F2 r = fma2(acc, e, add2(acc, e));
+    return F2{fminf(r.x, 0x1p124f), fminf(r.y, 0x1p124f)};
+  }
   __device__ static float close(float acc) {
     const float a = rcp_fast(1.0f + acc);
     return acc <= 1.0f ? acc * a : -a;
@@ -119,17 +145,49 @@ struct LeakyForm {
     return -((is_a(c) ? -c : 1.0f - c) * (is_a(d) ? -d : 1.0f - d));
   }
   __device__ static float step(float h, float c, float x) {
-    if (!FINE) return fmaf(c, x - h, h);
     const bool fast = is_a(c);  // x + a (h - x), else h + q (x - h)
     const float base = fast ? x : h;
     return fmaf(fabsf(c), (fast ? h : x) - base, base);
   }
-  __device__ static float back(float g, float c) { return FINE && is_a(c) ? -c * g : fmaf(-c, g, g); }
-  __device__ static float dx(float g, float c) { return FINE && is_a(c) ? fmaf(c, g, g) : c * g; }
-  __device__ static float grad_base(float h, float x) { return h - x; }
-  __device__ static float dgate(float g, float c, float base) {
-    const float s = FINE ? fabsf(c) : c;
-    return g * base * fmaf(-s, s, s);
+  __device__ static F2 step(F2 h, F2 c, F2 x) { return F2{step(h.x, c.x, x.x), step(h.y, c.y, x.y)}; }
+  __device__ static float back(float g, float c) { return is_a(c) ? -c * g : fmaf(-c, g, g); }
+  __device__ static F2 back(F2 g, F2 c) { return F2{back(g.x, c.x), back(g.y, c.y)}; }
+  __device__ static float dx(float g, float c) { return is_a(c) ? fmaf(c, g, g) : c * g; }
+  __device__ static F2 base(F2 h, F2 x) { return sub2(h, x); }
+  __device__ static F2 grads(F2 g, F2 c, F2 base, F2* dx_, F2* dgate) {
+    const F2 s = F2{fabsf(c.x), fabsf(c.y)};
+    *dx_ = F2{dx(g.x, c.x), dx(g.y, c.y)};
+    *dgate = mul2(mul2(g, base), sub2(s, mul2(s, s)));
+    return back(g, c);
+  }
+};
+
+// Leaky form, 16-bit tensors: a decay is Q = 1 - A, and exp the hardware's.  A
+// slow channel is as exact as above; a fast one's result is off by a rounding
+// of the state before it, and the weights are off by some 2^-21, far below the
+// 2^-9 or 2^-12 that the tensors carry.  It takes half the instructions, and
+// the 16-bit kernels are bound by those, the fp32 ones by memory.
+struct LeakyHalfForm {
+  __device__ static float kept_gate() { return __int_as_float(0x7f800000); }
+  __device__ static float kept() { return 0.0f; }
+  __device__ static float open() { return 0.0f; }
+  __device__ static float coeff(float gate) { return rcp_fast(1.0f + ex2_fast(gate * 1.4426950409f)); }
+  __device__ static F2 coeff(F2 gate, F2*) {
+    const F2 t = mul2(gate, two(1.4426950409f)), d = add2(F2{ex2_fast(t.x), ex2_fast(t.y)}, two(1.0f));
+    return F2{rcp_fast(d.x), rcp_fast(d.y)};
+  }
+  __device__ static F2 more(F2 acc, F2 c, F2) { return step(acc, c, two(1.0f)); }
+  __device__ static float close(float acc) { return acc; }
+  __device__ static float apply(float c, float h, float H) { return fmaf(-c, h, h) + H; }
+  __device__ static float join(float c, float d) { return fmaf(-c, d, c) + d; }
+  __device__ static float step(float h, float c, float x) { return fmaf(c, x - h, h); }
+  __device__ static F2 step(F2 h, F2 c, F2 x) { return fma2(c, sub2(x, h), h); }
+  __device__ static F2 back(F2 g, F2 c) { return sub2(g, mul2(c, g)); }
+  __device__ static F2 base(F2 h, F2 x) { return sub2(h, x); }
+  __device__ static F2 grads(F2 g, F2 c, F2 base, F2* dx, F2* dgate) {
+    *dx = mul2(c, g);
+    *dgate = mul2(*dx, mul2(base, sub2(two(1.0f), c)));
+    return sub2(g, *dx);
   }
 };
 
@@ -158,6 +216,11 @@ constexpr int kRecMaxCluster = 16;
 template <int V>
 struct Cols {
   float v[V];
+  __device__ __forceinline__ F2 pair(int i) const { return F2{v[2 * i], v[2 * i + 1]}; }
+  __device__ __forceinline__ void pair(int i, F2 p) {
+    v[2 * i] = p.x;
+    v[2 * i + 1] = p.y;
+  }
 };
 
 template <int V, bool ALIGNED>
@@ -225,11 +288,11 @@ struct RecSpot {
   int n, steps, room;
 };
 
+// `len`: the valid steps of row q->b; the spot's n channels and t0 are set.
 template <int S>
-__device__ __forceinline__ void rec_extent(const RecArgs& a, int cols, RecSpot* q) {
-  q->n = (int)min64(a.D - q->col, cols);
-  q->steps = (int)max64(min64(rec_len(a, q->b) - q->t0, S), 0);
-  q->room = (int)max64(min64(a.L - q->t0, S), 0);
+__device__ __forceinline__ void rec_extent(int64_t len, int64_t L, RecSpot* q) {
+  q->steps = (int)max64(min64(len - q->t0, S), 0);
+  q->room = (int)max64(min64(L - q->t0, S), 0);
 }
 
 // An input may be fetched ahead where a lane's piece is what cp.async moves.
@@ -281,7 +344,7 @@ __device__ __forceinline__ void rec_take(Cols<V>* v, const E* stage, const void*
 }
 
 template <typename E, int V, int S, bool ALIGNED>
-constexpr size_t rec_stage_bytes(int tensors) {
+__host__ __device__ constexpr size_t rec_stage_bytes(int tensors) {
   return rec_ahead<E, V, ALIGNED>() ? (size_t)tensors * kRecWarps * S * 32 * V * sizeof(E) : 0;
 }
 
@@ -345,11 +408,12 @@ __device__ __forceinline__ void rec_reduce(Cols<V>* c, const Cols<V>* u, Cols<V>
 #pragma unroll
   for (int j = 0; j < S; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float e;
-      c[j].v[i] = Form::coeff(c[j].v[i], &e);
-      H->v[i] = Form::step(H->v[i], c[j].v[i], u[j].v[i]);
-      A->v[i] = Form::more(A->v[i], c[j].v[i], e);
+    for (int i = 0; i < V / 2; ++i) {
+      F2 e;
+      const F2 d = Form::coeff(c[j].pair(i), &e);
+      c[j].pair(i, d);
+      H->pair(i, Form::step(H->pair(i), d, u[j].pair(i)));
+      A->pair(i, Form::more(A->pair(i), d, e));
     }
 #pragma unroll
   for (int i = 0; i < V; ++i) A->v[i] = Form::close(A->v[i]);
@@ -360,7 +424,7 @@ __device__ __forceinline__ void rec_coeffs(Cols<V>* c) {
 #pragma unroll
   for (int j = 0; j < S; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) c[j].v[i] = Form::coeff(c[j].v[i]);
+    for (int i = 0; i < V / 2; ++i) c[j].pair(i, Form::coeff(c[j].pair(i), nullptr));
 }
 
 // The gradient's map of the warp's steps (its decay is A too).
@@ -370,7 +434,7 @@ __device__ __forceinline__ Cols<V> rec_reduce_back(const Cols<V>* c, const Cols<
 #pragma unroll
   for (int j = S - 1; j >= 0; --j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) G.v[i] = Form::back(g[j].v[i] + G.v[i], c[j].v[i]);
+    for (int i = 0; i < V / 2; ++i) G.pair(i, Form::back(add2(g[j].pair(i), G.pair(i)), c[j].pair(i)));
   return G;
 }
 
@@ -382,8 +446,11 @@ __device__ __forceinline__ void rec_run_forward(const RecArgs& a, const RecSpot&
 #pragma unroll
   for (int j = 0; j < S; ++j) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) h->v[i] = Form::step(h->v[i], c[j].v[i], u[j].v[i]);
-    if (j < q.room) rec_store<V, ALIGNED>(out, lane, q.n, j < q.steps ? *h : cols_of<V>(0.0f));
+    for (int i = 0; i < V / 2; ++i) h->pair(i, Form::step(h->pair(i), c[j].pair(i), u[j].pair(i)));
+    if (j < q.steps)
+      rec_store<V, ALIGNED>(out, lane, q.n, *h);
+    else if (j < q.room)
+      rec_store<V, ALIGNED>(out, lane, q.n, cols_of<V>(0.0f));
     out += a.h_t;
   }
 }
@@ -394,10 +461,10 @@ __device__ __forceinline__ void rec_replay(const Cols<V>* c, Cols<V>* u, Cols<V>
 #pragma unroll
   for (int j = 0; j < S; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float before = h.v[i];
-      h.v[i] = Form::step(before, c[j].v[i], u[j].v[i]);
-      u[j].v[i] = Form::grad_base(before, u[j].v[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      const F2 before = h.pair(i);
+      h.pair(i, Form::step(before, c[j].pair(i), u[j].pair(i)));
+      u[j].pair(i, Form::base(before, u[j].pair(i)));
     }
 }
 
@@ -411,17 +478,19 @@ __device__ __forceinline__ void rec_run_back(const RecArgs& a, const RecSpot& q,
 #pragma unroll
   for (int j = S - 1; j >= 0; --j) {
     Cols<V> ox, og;
-    const bool on = j < q.steps;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float total = g[j].v[i] + later->v[i];
-      ox.v[i] = on ? Form::dx(total, c[j].v[i]) : 0.0f;
-      og.v[i] = on ? Form::dgate(total, c[j].v[i], u[j].v[i]) : 0.0f;
-      later->v[i] = Form::back(total, c[j].v[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      F2 px, pg;
+      later->pair(i, Form::grads(add2(g[j].pair(i), later->pair(i)), c[j].pair(i), u[j].pair(i), &px, &pg));
+      ox.pair(i, px);
+      og.pair(i, pg);
     }
-    if (j < q.room) {
+    if (j < q.steps) {
       rec_store<V, ALIGNED>(dx, lane, q.n, ox);
       rec_store<V, ALIGNED>(dg, lane, q.n, og);
+    } else if (j < q.room) {
+      rec_store<V, ALIGNED>(dx, lane, q.n, cols_of<V>(0.0f));
+      rec_store<V, ALIGNED>(dg, lane, q.n, cols_of<V>(0.0f));
     }
     dx -= a.o_t;
     dg -= a.o_t;
@@ -437,8 +506,9 @@ __device__ __forceinline__ RecSpot rec_short_spot(const RecArgs& a, const RecPla
   if (chain >= p.chains) return q;
   q.b = chain / p.groups;
   q.col = (chain - q.b * p.groups) * 128;
+  q.n = (int)min64(a.D - q.col, 128);
   q.t0 = (warp % p.wt) * S;
-  rec_extent<S>(a, 128, &q);
+  rec_extent<S>(rec_len(a, q.b), a.L, &q);
   return q;
 }
 
@@ -518,39 +588,25 @@ __global__ void __launch_bounds__(kRecThreads, 2) recurrence_short_backward_kern
 }
 
 // ---- longer sequences: one cluster of K blocks per chain walks along time,
-// K tiles of 8 S steps at once.  The tiles' maps are exchanged through the
-// cluster's shared memory; every block applies all of them in time order, so
-// each knows the state in front of its own tile and the one behind them all,
-// which it carries on: no block waits for another cluster, x and gate are
-// read once however few chains there are, and the order of every sum is fixed.
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
-  uint32_t there;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-  return v;
-}
+// K tiles of 8 S steps at once.  Every block sends its tile's map to all of
+// them (stores to the cluster's shared memory that count bytes on the
+// receiver's barrier) and applies all K in time order, so each knows the state
+// in front of its own tile and the one behind them all, which it carries on:
+// no block waits for another cluster, x and gate are read once however few
+// chains there are, and the order of every sum is fixed.
+struct RecMeeting {
+  float2* maps;  // [2][K][32 V] (A, H) by parity of the round and rank, behind the stages
+  uint64_t* bar; // [2]
+  int* abort;
+};
 
-// Thread < 32 V: its channel's part of joining the tiles.  `share` publishes
-// the block's map (of the warps' maps, in time order or in reverse) in
-// `mine`[2][32 V]; after the cluster's barrier, `meet` applies the K maps (in
-// the order of ranks, or in reverse) to `state`, the one in front of them all,
-// returns the one in front of this block's tile and moves `state` behind them.
+constexpr size_t rec_meeting_bytes(int V, int K) { return K > 1 ? (size_t)2 * K * 32 * V * sizeof(float2) : 0; }
+
+// Sends a block's map (of the warps' maps, in time order or in reverse), this
+// thread's channel c, to every block's maps[parity][rank].
 template <typename Form, int V>
-__device__ __forceinline__ void rec_share(const float (*mA)[32 * V], const float (*mH)[32 * V], bool reverse,
-                                          float* mine, int c) {
+__device__ __forceinline__ void rec_send(const RecMeeting& m, const float (*mA)[32 * V], const float (*mH)[32 * V],
+                                         bool reverse, int parity, int rank, int K, int c) {
   float A = Form::kept(), H = 0.0f;
 #pragma unroll
   for (int k = 0; k < kRecWarps; ++k) {
@@ -558,75 +614,115 @@ __device__ __forceinline__ void rec_share(const float (*mA)[32 * V], const float
     H = Form::apply(mA[w][c], H, mH[w][c]);
     A = Form::join(A, mA[w][c]);
   }
-  mine[c] = A;
-  mine[32 * V + c] = H;
+  const uint32_t at = smem_u32(m.maps + (parity * K + rank) * 32 * V + c), bar = smem_u32(m.bar + parity);
+  if (c == 0) mbar_arrive_expect_tx(m.bar + parity, (uint32_t)(K * 32 * V * sizeof(float2)));
+  for (int k = 0; k < K; ++k) {
+    uint32_t there, there_bar;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(k));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there_bar) : "r"(bar), "r"(k));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(there),
+                 "f"(A), "f"(H), "r"(there_bar)
+                 : "memory");
+  }
 }
 
+// Applies the K maps of a round (in the order of ranks, or in reverse) to
+// `state`, the one in front of them all; returns the one in front of this
+// block's tile and moves `state` behind them.  A sender overwrites a map two
+// rounds later, after it has received this block's map of the round between,
+// which this thread sends when it is done here.
 template <typename Form, int V>
-__device__ __forceinline__ float rec_meet(const float* mine, bool reverse, int rank, int K, int c, float* state) {
-  const uint32_t at = smem_u32(mine + c);
+__device__ __forceinline__ float rec_meet(const RecMeeting& m, bool reverse, int round, int rank, int K, int c,
+                                          float* state) {
+  mbar_wait<true>(m.bar + (round & 1), (round >> 1) & 1, m.abort, SPK_DEV_PIPE_TIMEOUT);
+  const float2* maps = m.maps + (round & 1) * K * 32 * V + c;
   float s = *state, front = s;
 #pragma unroll 4
   for (int k = 0; k < K; ++k) {
     const int r = reverse ? K - 1 - k : k;
-    const float A = cluster_load(at, r), H = cluster_load(at + 4 * 32 * V, r);
+    const float2 v = maps[r * 32 * V];
     if (r == rank) front = s;
-    s = Form::apply(A, s, H);
+    s = Form::apply(v.x, s, v.y);
   }
   *state = s;
   return front;
 }
 
-template <int V, int S>
-__device__ __forceinline__ RecSpot rec_long_spot(const RecArgs& a, const RecPlan& p, int64_t chain, int64_t chunk,
-                                                 int warp) {
-  RecSpot q{};
-  q.b = chain / p.groups;
-  q.col = (chain - q.b * p.groups) * (32 * V);
-  q.t0 = (chunk * kRecWarps + warp) * S;
-  if (chunk < 0 || chunk >= p.chunks) return q;  // nothing there: the state stays
-  rec_extent<S>(a, 32 * V, &q);
-  return q;
+__device__ __forceinline__ void rec_meeting_open(const RecMeeting& m, int K) {
+  if (K == 1) return;
+  if (threadIdx.x == 0) {
+    mbar_init(m.bar, 1);
+    mbar_init(m.bar + 1, 1);
+    *m.abort = 0;
+    fence_barrier_init();
+  }
+  cluster_sync_all();
 }
+
+// The chain of a cluster, and a warp's spot in the tile `chunk` of it.
+template <int V, int S>
+struct RecChain {
+  int64_t len, L;
+  RecSpot q;
+  int n;
+
+  __device__ __forceinline__ RecChain(const RecArgs& a, const RecPlan& p, int64_t chain) : L(a.L) {
+    q.b = chain / p.groups;
+    q.col = (chain - q.b * p.groups) * (32 * V);
+    n = (int)min64(a.D - q.col, 32 * V);
+    len = rec_len(a, q.b);
+  }
+  __device__ __forceinline__ RecSpot at(int64_t chunk, int warp) const {
+    RecSpot r = q;
+    r.t0 = (chunk * kRecWarps + warp) * S;
+    r.n = n;
+    if (chunk >= 0)
+      rec_extent<S>(len, L, &r);
+    else
+      r.steps = r.room = 0;  // in front of the first tile; behind the last, no step is left either
+    return r;
+  }
+};
 
 template <typename E, typename Form, int V, int S, bool ALIGNED>
 __global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_kernel(RecArgs a, RecPlan p) {
   extern __shared__ __align__(16) unsigned char rec_smem[];
-  __shared__ __align__(16) float mA[2][kRecWarps][32 * V], mH[2][kRecWarps][32 * V], mine[2][2 * 32 * V], sC[32 * V];
+  __shared__ __align__(16) float mA[2][kRecWarps][32 * V], mH[2][kRecWarps][32 * V], sC[32 * V];
+  __shared__ uint64_t bars[2];
+  __shared__ int abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = threadIdx.x;
-  const int rank = (int)cluster_rank(), K = (int)cluster_size();
+  const int rank = (int)cluster_ctarank(), K = p.cluster;
   const int64_t chain = blockIdx.x / K;
+  const RecMeeting meeting{reinterpret_cast<float2*>(rec_smem + rec_stage_bytes<E, V, S, ALIGNED>(2)), bars, &abort};
+  rec_meeting_open(meeting, K);
   const RecInputs<E, V, S, ALIGNED> in(rec_smem, warp, lane);
-  RecSpot q = rec_long_spot<V, S>(a, p, chain, rank, warp);
+  const RecChain<V, S> walk(a, p, chain);
+  RecSpot q = walk.at(rank, warp);
   in.ask(a, q, Form::kept_gate(), false);
-  const int width = (int)min64(a.D - q.col, 32 * V), ch = rec_col<V, ALIGNED>(slot / V, slot % V);
+  const int width = walk.n, ch = rec_col<V, ALIGNED>(slot / V, slot % V);
   const bool joins = slot < 32 * V;  // this thread joins the tiles for channel ch
   float state = joins && ch < width && a.h0 != nullptr ? a.h0[q.b * a.D + q.col + ch] : 0.0f;
   int round = 0;
-  for (int64_t first = 0; first < p.chunks; first += K, round ^= 1) {
+  for (int64_t first = 0; first < p.chunks; first += K, ++round) {
     const int64_t chunk = first + rank;
     Cols<V> c[S], u[S], A, H;
     in.wait();
     in.gate(a, q, c, Form::kept_gate());
     in.x(a, q, u);
-    const RecSpot next = rec_long_spot<V, S>(a, p, chain, chunk + K, warp);
+    const RecSpot next = walk.at(chunk + K, warp);
     in.ask(a, next, Form::kept_gate(), false);
     rec_reduce<Form, V, S>(c, u, &A, &H);
-    cols_st<V>(mA[round][warp], lane, A);
-    cols_st<V>(mH[round][warp], lane, H);
+    cols_st<V>(mA[round & 1][warp], lane, A);
+    cols_st<V>(mH[round & 1][warp], lane, H);
     __syncthreads();
-    if (K > 1) {
-      if (joins) rec_share<Form, V>(mA[round], mH[round], false, mine[round], slot);
-      cluster_arrive();
-      cluster_wait();
-    }
     if (joins) {
       float front = state;
       if (K > 1) {
-        front = rec_meet<Form, V>(mine[round], false, rank, K, slot, &state);
+        rec_send<Form, V>(meeting, mA[round & 1], mH[round & 1], false, round & 1, rank, K, slot);
+        front = rec_meet<Form, V>(meeting, false, round, rank, K, slot, &state);
       } else {
 #pragma unroll
-        for (int k = 0; k < kRecWarps; ++k) state = Form::apply(mA[round][k][slot], state, mH[round][k][slot]);
+        for (int k = 0; k < kRecWarps; ++k) state = Form::apply(mA[round & 1][k][slot], state, mH[round & 1][k][slot]);
       }
       sC[slot] = front;
       if (a.carry != nullptr && chunk > 0 && chunk < p.chunks && ch < width)
@@ -634,15 +730,12 @@ __global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_kernel(RecArgs
     }
     __syncthreads();
     Cols<V> h = cols_ld<V>(sC, lane);
-    for (int k = 0; k < warp; ++k) cols_apply<Form, V>(mA[round][k], mH[round][k], lane, &h);
+    for (int k = 0; k < warp; ++k) cols_apply<Form, V>(mA[round & 1][k], mH[round & 1][k], lane, &h);
     rec_run_forward<E, Form, V, S, ALIGNED>(a, q, c, u, &h, lane);
     q = next;
   }
   if (joins && rank == 0 && ch < width) a.last[q.b * a.D + q.col + ch] = state;
-  if (K > 1) {  // the maps of this block may still be read
-    cluster_arrive();
-    cluster_wait();
-  }
+  if (K > 1) cluster_sync_all();  // maps may still be on their way here
 }
 
 // Backward: the same tiles from the end.  A tile runs its steps forward from
@@ -653,26 +746,31 @@ template <typename E, typename Form, int V, int S, bool ALIGNED>
 __global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_backward_kernel(RecArgs a, RecPlan p) {
   extern __shared__ __align__(16) unsigned char rec_smem[];
   __shared__ __align__(16) float mA[kRecWarps][32 * V], mH[kRecWarps][32 * V], mG[kRecWarps][32 * V];
-  __shared__ __align__(16) float mine[2][2 * 32 * V], sC[32 * V];
+  __shared__ __align__(16) float sC[32 * V];
+  __shared__ uint64_t bars[2];
+  __shared__ int abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = threadIdx.x;
-  const int rank = (int)cluster_rank(), K = (int)cluster_size();
+  const int rank = (int)cluster_ctarank(), K = p.cluster;
   const int64_t chain = blockIdx.x / K;
+  const RecMeeting meeting{reinterpret_cast<float2*>(rec_smem + rec_stage_bytes<E, V, S, ALIGNED>(3)), bars, &abort};
+  rec_meeting_open(meeting, K);
   const RecInputs<E, V, S, ALIGNED> in(rec_smem, warp, lane);
   const int64_t top = (p.chunks - 1) / K * K;
-  RecSpot q = rec_long_spot<V, S>(a, p, chain, top + rank, warp);
+  const RecChain<V, S> walk(a, p, chain);
+  RecSpot q = walk.at(top + rank, warp);
   in.ask(a, q, Form::kept_gate(), true);
-  const int width = (int)min64(a.D - q.col, 32 * V), ch = rec_col<V, ALIGNED>(slot / V, slot % V);
+  const int width = walk.n, ch = rec_col<V, ALIGNED>(slot / V, slot % V);
   const bool joins = slot < 32 * V;
   float state = joins && ch < width && a.glast != nullptr ? a.glast[q.b * a.D + q.col + ch] : 0.0f;
   int round = 0;
-  for (int64_t first = top; first >= 0; first -= K, round ^= 1) {
+  for (int64_t first = top; first >= 0; first -= K, ++round) {
     const int64_t chunk = first + rank;
     Cols<V> c[S], u[S], g[S], h;
     in.wait();
     in.gate(a, q, c, Form::kept_gate());
     in.x(a, q, u);
     in.gh(a, q, g);
-    const RecSpot next = rec_long_spot<V, S>(a, p, chain, chunk - K, warp);
+    const RecSpot next = walk.at(chunk - K, warp);
     in.ask(a, next, Form::kept_gate(), true);
     {
       Cols<V> A, H;
@@ -683,19 +781,15 @@ __global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_backward_kerne
     }
     h = cols_of<V>(0.0f);
     const float* start = chunk > 0 ? a.carry + ((chunk - 1) * a.B + q.b) * a.D : a.h0 + q.b * a.D;
-    if (chunk > 0 || a.h0 != nullptr) h = rec_load<V, ALIGNED>(start + q.col, lane, q.n, 0.0f);
+    if (chunk < p.chunks && (chunk > 0 || a.h0 != nullptr)) h = rec_load<V, ALIGNED>(start + q.col, lane, q.n, 0.0f);
     __syncthreads();
-    if (K > 1) {
-      if (joins) rec_share<Form, V>(mA, mG, true, mine[round], slot);
-      cluster_arrive();
-    }
+    if (K > 1 && joins) rec_send<Form, V>(meeting, mA, mG, true, round & 1, rank, K, slot);
     for (int k = 0; k < warp; ++k) cols_apply<Form, V>(mA[k], mH[k], lane, &h);
     rec_replay<Form, V, S>(c, u, h);
-    if (K > 1) cluster_wait();
     if (joins) {
       float front = state;
       if (K > 1) {
-        front = rec_meet<Form, V>(mine[round], true, rank, K, slot, &state);
+        front = rec_meet<Form, V>(meeting, true, round, rank, K, slot, &state);
       } else {
 #pragma unroll
         for (int k = kRecWarps - 1; k >= 0; --k) state = Form::apply(mA[k][slot], state, mG[k][slot]);
@@ -710,10 +804,7 @@ __global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_backward_kerne
     q = next;
   }
   if (joins && rank == 0 && ch < width && a.dh0 != nullptr) a.dh0[q.b * a.D + q.col + ch] = state;
-  if (K > 1) {  // the maps of this block may still be read
-    cluster_arrive();
-    cluster_wait();
-  }
+  if (K > 1) cluster_sync_all();  // maps may still be on their way here
 }
 
 // One step of the recurrence over n cells: out (element type) and the new
@@ -733,8 +824,10 @@ template <typename E, typename F>
 inline void with_form(int form, F&& f) {
   if (form == SPK_REC_GATE)
     f(GateForm{});
+  else if constexpr (sizeof(E) == 4)
+    f(LeakyForm{});
   else
-    f(LeakyForm<sizeof(E) == 4>{});
+    f(LeakyHalfForm{});
 }
 
 // Shape, type and alignment checks shared by the recurrence's entry points.
@@ -755,23 +848,26 @@ static bool rec_aligned(const void* p, size_t eb, int64_t stride_b, int64_t stri
   return aligned_to(p, 4 * eb) && stride_b % 4 == 0 && stride_t % 4 == 0;
 }
 
-// Channels per chain of a long recurrence: 128 (tiles of 64 steps), or 32
-// (tiles of 256) when clusters of 128-channel chains would leave most of the
-// GPU idle.
-static int rec_long_cols(int64_t B, int64_t D) {
-  return B * ceil_div(D, 128) * kRecMaxCluster >= 128 ? 128 : 32;
+// Channels per chain of a long recurrence, V = 4 or 2 per lane: 128 (tiles of
+// 64 steps) or 64 (tiles of 128 steps: twice the chains, half the joins).
+// Forward + backward, us, 128 against 64 channels:
+//   bf16  1x32768x512: 218 / 194   4x32768x512: 380 / 389   64x2048x512: 253 / 348
+//   fp32  4x32768x512: 746 / 550   16x8192x512: 707 / 520   64x2048x512: 535 / 495
+// (fp32's backward stages leave room for one block per SM beside 128-channel maps).
+static int rec_long_cols(int dtype, int64_t B, int64_t D) {
+  return dtype == SPK_F32 || B * ceil_div(D, 128) < 16 ? 64 : 128;
 }
 
-static int64_t rec_chunk(int64_t B, int64_t L, int64_t D) {
-  return L <= 64 ? 64 : 64 * (128 / rec_long_cols(B, D));
+static int64_t rec_chunk(int dtype, int64_t B, int64_t L, int64_t D) {
+  return L <= 64 ? 64 : 64 * (128 / rec_long_cols(dtype, B, D));
 }
 
 // Batch rows that follow one another like channels (no lengths, batch stride D
 // everywhere) become channels first, so that narrow rows share a warp.
-static RecPlan rec_plan(RecArgs* a, bool merge) {
+static RecPlan rec_plan(RecArgs* a, int dtype, bool merge) {
   RecPlan p{};
-  const int64_t chunk = rec_chunk(a->B, a->L, a->D);
-  p.cols = a->L <= 64 ? 128 : rec_long_cols(a->B, a->D);
+  const int64_t chunk = rec_chunk(dtype, a->B, a->L, a->D);
+  p.cols = a->L <= 64 ? 128 : rec_long_cols(dtype, a->B, a->D);
   if (merge && a->lengths == nullptr) {
     a->D *= a->B;
     a->B = 1;
@@ -802,14 +898,15 @@ struct RecOccupancy {
 };
 
 template <typename K>
-static cudaError_t rec_occupancy(K* kernel, size_t smem, RecOccupancy* out) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+static cudaError_t rec_occupancy(K* kernel, int V, size_t stages, RecOccupancy* out) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)(stages + rec_meeting_bytes(V, kRecMaxCluster)));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   for (int k = 1; k <= kRecMaxCluster && e == cudaSuccess; ++k) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)k);
     cfg.blockDim = dim3(kRecThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = stages + rec_meeting_bytes(V, k);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)k;
@@ -830,25 +927,27 @@ template <typename E, typename Form, int V, int S, bool ALIGNED, bool BACKWARD>
 static cudaError_t rec_launch_long(const RecArgs& a, const RecPlan& p, cudaStream_t st) {
   auto* const kernel = BACKWARD ? recurrence_long_backward_kernel<E, Form, V, S, ALIGNED>
                                 : recurrence_long_kernel<E, Form, V, S, ALIGNED>;
-  const size_t smem = rec_stage_bytes<E, V, S, ALIGNED>(BACKWARD ? 3 : 2);
+  const size_t stages = rec_stage_bytes<E, V, S, ALIGNED>(BACKWARD ? 3 : 2);
   static PerDevice<RecOccupancy> cache;  // one per kernel
   RecOccupancy occ;
-  cudaError_t e = cache.get(&occ, [&](RecOccupancy* o) { return rec_occupancy(kernel, smem, o); });
+  cudaError_t e = cache.get(&occ, [&](RecOccupancy* o) { return rec_occupancy(kernel, V, stages, o); });
   if (e != cudaSuccess) return e;
   // The fewest blocks per chain that need the fewest rounds: every cluster
   // takes ceil(chunks / k) rounds, as many clusters at once as fit.
-  int cluster = 1;
+  RecPlan plan = p;
+  plan.cluster = 1;
   int64_t best = 0;
   for (int k = 1; k <= kRecMaxCluster && k <= p.chunks; ++k) {
     if (occ.clusters[k] <= 0) continue;
     const int64_t rounds = ceil_div(p.chains, occ.clusters[k]) * ceil_div(p.chunks, k);
     if (best == 0 || rounds < best) {
       best = rounds;
-      cluster = k;
+      plan.cluster = k;
     }
   }
-  return launch_dependent_cluster(kernel, dim3((unsigned)(p.chains * cluster)), dim3(kRecThreads), smem, st,
-                                  (unsigned)cluster, false, a, p);
+  return launch_dependent_cluster(kernel, dim3((unsigned)(p.chains * plan.cluster)), dim3(kRecThreads),
+                                  stages + rec_meeting_bytes(V, plan.cluster), st, (unsigned)plan.cluster, false, a,
+                                  plan);
 }
 
 template <typename E, typename Form, int V, int S, bool ALIGNED>
@@ -864,8 +963,9 @@ static int rec_run(bool backward, int dtype, int form, bool aligned, const RecAr
     using E = decltype(e);
     with_form<E>(form, [&](auto f) {
       using F = decltype(f);
-      if (a.L > 64 && p.cols == 32)
-        rc = rec_launch_long<E, F, 1, 32, true>(backward, a, p, st);
+      if (a.L > 64 && p.cols == 64)
+        rc = aligned ? rec_launch_long<E, F, 2, 16, true>(backward, a, p, st)
+                     : rec_launch_long<E, F, 2, 16, false>(backward, a, p, st);
       else if (a.L > 64)
         rc = aligned ? rec_launch_long<E, F, 4, 8, true>(backward, a, p, st)
                      : rec_launch_long<E, F, 4, 8, false>(backward, a, p, st);
@@ -884,8 +984,8 @@ static int rec_run(bool backward, int dtype, int form, bool aligned, const RecAr
 
 }  // namespace spk
 
-extern "C" int64_t spk_recurrence_chunk(int64_t B, int64_t L, int64_t D) {
-  return B > 0 && L > 0 && D > 0 ? spk::rec_chunk(B, L, D) : 64;
+extern "C" int64_t spk_recurrence_chunk(int dtype, int64_t B, int64_t L, int64_t D) {
+  return B > 0 && L > 0 && D > 0 ? spk::rec_chunk(dtype, B, L, D) : 64;
 }
 
 extern "C" int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_stride_t, const void* gate,
@@ -923,7 +1023,7 @@ extern "C" int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_strid
                        spk::rec_aligned(h, eb, h_stride_b, h_stride_t) && spk::aligned_to(state, 16) &&
                        spk::aligned_to(last, 16) && spk::aligned_to(carry, 16);
   cudaStream_t st = (cudaStream_t)stream;
-  const spk::RecPlan p = spk::rec_plan(&a, x_stride_b == D && g_stride_b == D && h_stride_b == D);
+  const spk::RecPlan p = spk::rec_plan(&a, dtype, x_stride_b == D && g_stride_b == D && h_stride_b == D);
   return spk::rec_run(false, dtype, form, aligned, a, p, st);
 }
 
@@ -938,8 +1038,8 @@ extern "C" int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_
   if (B == 0 || D == 0) return SPK_OK;
   SPK_REQUIRE(L == 0 || (x != nullptr && gate != nullptr && dx != nullptr && dgate != nullptr),
               "x, gate, dx and dgate must be non-null");
-  SPK_REQUIRE(L <= spk::rec_chunk(B, L, D) || carry != nullptr, "the forward pass's carry is needed above %lld steps",
-              (long long)spk::rec_chunk(B, L, D));
+  SPK_REQUIRE(L <= spk::rec_chunk(dtype, B, L, D) || carry != nullptr, "the forward pass's carry is needed above %lld steps",
+              (long long)spk::rec_chunk(dtype, B, L, D));
   SPK_REQUIRE(spk::aligned_to(x, eb) && spk::aligned_to(gate, eb) && spk::aligned_to(gh, eb) &&
                   spk::aligned_to(dx, eb) && spk::aligned_to(dgate, eb) && spk::aligned_to(state, 4) &&
                   spk::aligned_to(lengths, 4) && spk::aligned_to(carry, 4) && spk::aligned_to(glast, 4) &&
@@ -975,7 +1075,7 @@ extern "C" int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_
                        spk::aligned_to(glast, 16) && spk::aligned_to(carry, 16) && spk::aligned_to(dstate, 16);
   cudaStream_t st = (cudaStream_t)stream;
   const spk::RecPlan p = spk::rec_plan(
-      &a, x_stride_b == D && g_stride_b == D && d_stride_b == D && (gh == nullptr || gh_stride_b == D));
+      &a, dtype, x_stride_b == D && g_stride_b == D && d_stride_b == D && (gh == nullptr || gh_stride_b == D));
   return spk::rec_run(true, dtype, form, aligned, a, p, st);
 }
 

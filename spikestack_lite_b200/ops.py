@@ -667,7 +667,7 @@ def _recurrence_forward(x, gate, state, form, dim, lengths, keep):
     last = torch.empty_like(state)
     carry = None
     if keep:
-        chunk = int(lib.spk_recurrence_chunk(B, L, D))
+        chunk = int(lib.spk_recurrence_chunk(_DTYPES[x.dtype], B, L, D))
         if L > chunk:
             carry = torch.empty((L + chunk - 1) // chunk - 1, B, D, dtype=torch.float32, device=x.device)
     _call(x, "spk_recurrence", ptr(x), xb, xt, ptr(gate), gb, gt, _DTYPES[x.dtype], form, B, L, D, ptr(state),

@@ -90,7 +90,7 @@ def test_recurrence_entry_points_reject_bad_arguments(lib):
 
     assert bwd(B=0) == SPK_OK
     for bad in (dict(dtype=3), dict(form=-1), dict(dx=None), dict(dgate=None), dict(x=None), dict(gh=ODD),
-                dict(glast=ODD), dict(L=lib.spk_recurrence_chunk(2, 1 << 20, 8) + 1)):
+                dict(glast=ODD), dict(L=lib.spk_recurrence_chunk(0, 2, 1 << 20, 8) + 1)):
         assert bwd(**bad) == SPK_EINVAL, bad
     assert b"carry" in lib.spk_last_error()
 
