@@ -46,6 +46,19 @@ __device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& v) {
   *reinterpret_cast<Pack<E, V>*>(p) = v;
 }
 
+// The hardware's exponential of two and reciprocal (relative errors of 2^-22
+// and 2^-23; a subnormal argument or result becomes 0).
+__device__ __forceinline__ float ex2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 inline size_t elem_bytes(int dtype) { return dtype == SPK_F32 ? 4 : (dtype == SPK_BF16 || dtype == SPK_F16) ? 2 : 0; }
 
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

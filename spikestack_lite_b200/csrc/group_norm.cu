@@ -30,73 +30,40 @@ struct GnArgs {
   float* dbias;
   int64_t S, P;
   int C, G, cg;
-  int rows, tiles;      // positions per tile, tiles per sample
+  int tpr, rpp, threads;  // threads side by side and rows at once in a block
+  int k, rows, tiles;   // groups per block (resident); positions per tile (tiled); blocks per sample
+  int64_t parts;        // rows of `part`
   float eps, thr;
 };
 
-template <int ACT>
+constexpr int kGnThreads = 256;
+
+// sigmoid for an output of type E: the accurate exponential for fp32, the
+// hardware's (2^-21 relative) for 16-bit elements.
+template <typename E>
+__device__ __forceinline__ float gn_sigmoid(float z) {
+  return rcp_fast(1.0f + (sizeof(E) == 4 ? expf(-z) : ex2_fast(z * -1.4426950409f)));
+}
+
+template <typename E, int ACT>
 __device__ __forceinline__ float gn_act(float z, float thr) {
   if (ACT == SPK_ACT_HEAVISIDE) return z - thr > 0.0f ? 1.0f : 0.0f;
-  if (ACT == SPK_ACT_SILU) return z * __fdividef(1.0f, 1.0f + expf(-z));
+  if (ACT == SPK_ACT_SILU) return z * gn_sigmoid<E>(z);
   return z;
 }
 
 // act'(z) gy
-template <int ACT>
+template <typename E, int ACT>
 __device__ __forceinline__ float gn_act_grad(float z, float thr, float gy) {
   if (ACT == SPK_ACT_HEAVISIDE) {
-    const float s = __fdividef(1.0f, 1.0f + expf(-10.0f * (z - thr)));
+    const float s = gn_sigmoid<E>(10.0f * (z - thr));
     return gy * s * (1.0f - s) * 10.0f;
   }
   if (ACT == SPK_ACT_SILU) {
-    const float s = __fdividef(1.0f, 1.0f + expf(-z));
+    const float s = gn_sigmoid<E>(z);
     return gy * (s * fmaf(z, 1.0f - s, 1.0f));
   }
   return gy;
-}
-
-struct Moments {
-  float n, mean, m2;
-};
-
-__device__ __forceinline__ Moments merge(const Moments& a, const Moments& b) {
-  Moments r;
-  r.n = a.n + b.n;
-  const float w = r.n > 0.0f ? __fdividef(b.n, r.n) : 0.0f;
-  const float d = b.mean - a.mean;
-  r.mean = fmaf(d, w, a.mean);
-  r.m2 = a.m2 + b.m2 + d * d * a.n * w;
-  return r;
-}
-
-constexpr int kGnThreads = 256;
-
-// Partial moments of one channel over the rows of one tile: thread = channel
-// (blockIdx.y tiles the channels), rows split over threadIdx.y.
-template <typename E>
-__global__ void __launch_bounds__(kGnThreads) gn_stats_kernel(GnArgs a) {
-  __shared__ Moments sm[8][32];
-  const int c = blockIdx.y * 32 + threadIdx.x;
-  const int64_t tile = blockIdx.x, s = tile / a.tiles;
-  const int64_t p0 = (tile - s * a.tiles) * a.rows, p1 = min64(p0 + a.rows, a.P);
-  Moments m{0.0f, 0.0f, 0.0f};
-  if (c < a.C) {
-    const E* x = static_cast<const E*>(a.x) + (s * a.P) * a.C + c;
-    for (int64_t p = p0 + threadIdx.y; p < p1; p += 8) {
-      m.n += 1.0f;
-      const float v = elem_to_f32(x[p * a.C]), d = v - m.mean;
-      m.mean += __fdividef(d, m.n);
-      m.m2 = fmaf(d, v - m.mean, m.m2);
-    }
-  }
-  sm[threadIdx.y][threadIdx.x] = m;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < a.C) {
-    for (int i = 1; i < 8; ++i) m = merge(m, sm[i][threadIdx.x]);
-    float* out = a.part + (tile * a.C + c) * 2;
-    out[0] = m.mean;
-    out[1] = m.m2;
-  }
 }
 
 __device__ __forceinline__ float gn_warp_sum(float v) {
@@ -105,112 +72,515 @@ __device__ __forceinline__ float gn_warp_sum(float v) {
   return v;
 }
 
-// One warp per (sample, group): merges the tiles' moments.
-__global__ void __launch_bounds__(kGnThreads) gn_stats_finish_kernel(GnArgs a) {
-  const int64_t u = (int64_t)blockIdx.x * (kGnThreads / 32) + (threadIdx.x >> 5);
-  if (u >= a.S * a.G) return;
+// A block's threads over a tile: V neighbouring channels each, `tpr` threads
+// side by side, `rpp` rows at once (the rest of the block idles).
+struct GnSpot {
+  int cv, r;  // the thread's first channel within the tile's columns, its first row
+  bool live;
+};
+
+__device__ __forceinline__ GnSpot gn_spot(int V, int tpr, int rpp) {
+  GnSpot q;
+  q.r = (int)threadIdx.x / tpr;
+  q.cv = ((int)threadIdx.x - q.r * tpr) * V;
+  q.live = q.r < rpp;
+  return q;
+}
+
+// Per-channel constants of the thread's V channels.
+template <int V>
+struct GnAffine {
+  float mean[V], rstd[V], w[V], b[V];
+};
+
+template <int V>
+__device__ __forceinline__ void gn_affine(const GnArgs& a, int64_t s, int c0, GnAffine<V>* f) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int64_t u = s * a.G + (c0 + j) / a.cg;
+    f->mean[j] = a.mean[u];
+    f->rstd[j] = a.rstd[u];
+    f->w[j] = a.weight != nullptr ? a.weight[c0 + j] : 1.0f;
+    f->b[j] = a.bias != nullptr ? a.bias[c0 + j] : 0.0f;
+  }
+}
+
+template <typename E, int ACT, int V>
+__device__ __forceinline__ Pack<E, V> gn_forward(const Pack<E, V>& x, const GnAffine<V>& f, float thr) {
+  Pack<E, V> y;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    y.e[j] = elem_from_f32<E>(
+        gn_act<E, ACT>(fmaf((elem_to_f32(x.e[j]) - f.mean[j]) * f.rstd[j], f.w[j], f.b[j]), thr));
+  return y;
+}
+
+// dz and xhat of one element.
+template <typename E, int ACT, int V>
+__device__ __forceinline__ float gn_dz(const Pack<E, V>& x, const Pack<E, V>& gy, const GnAffine<V>& f, int j,
+                                       float thr, float* xhat) {
+  *xhat = (elem_to_f32(x.e[j]) - f.mean[j]) * f.rstd[j];
+  return gn_act_grad<E, ACT>(fmaf(*xhat, f.w[j], f.b[j]), thr, elem_to_f32(gy.e[j]));
+}
+
+// ---- resident form: a block holds a sample's k groups (all positions) in
+// registers, so x (and gy) cross HBM once.  N packs of 16 bytes per thread.
+template <int N>
+__device__ __forceinline__ int gn_rows(const GnArgs& a, const GnSpot& q) {  // rows of this thread, at most N
+  return q.live ? (int)ceil_div(max64(a.P - q.r, 0), a.rpp) : 0;
+}
+
+template <typename E, int N, int V>
+__device__ __forceinline__ void gn_load(const E* p, int64_t step, int rows, Pack<E, V>* v) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < rows) v[i] = load_pack<E, V>(p + i * step);
+}
+
+// Mean and sum of squares about it of `rows` packs' channels j0 .. j0 + J - 1.
+template <typename E, int N, int V, int J>
+__device__ __forceinline__ float4 gn_moments(const Pack<E, V>* x, int rows, int j0) {
+  const float n = (float)(rows * J), inv = rows > 0 ? __fdividef(1.0f, n) : 0.0f;
+  float sum = 0.0f, m2 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < rows) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) sum += elem_to_f32(x[i].e[j0 + j]);
+    }
+  const float mean = sum * inv;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < rows) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const float d = elem_to_f32(x[i].e[j0 + j]) - mean;
+        m2 = fmaf(d, d, m2);
+      }
+    }
+  return make_float4(mean, m2, n, 0.0f);
+}
+
+// WHOLE: every pack lies in one group (cg is a multiple of V).
+template <typename E, int ACT, int N, bool WHOLE>
+__global__ void __launch_bounds__(kGnThreads, 2) gn_resident_kernel(GnArgs a) {
+  constexpr int V = 16 / (int)sizeof(E);
+  extern __shared__ __align__(16) unsigned char gn_smem[];
+  float4* const part = reinterpret_cast<float4*>(gn_smem);  // [groups][parts] mean, sum of squares about it, count
+  const int64_t s = blockIdx.x / a.tiles;
+  const int g0 = (int)(blockIdx.x - s * a.tiles) * a.k, ng = min(a.k, a.G - g0), width = ng * a.cg;
+  GnSpot q = gn_spot(V, a.tpr, a.rpp);
+  q.live = q.live && q.cv < width;
+  const int rows = gn_rows<N>(a, q), c0 = g0 * a.cg + q.cv;
+  const int64_t at = (s * a.P + q.r) * a.C + c0, step = (int64_t)a.rpp * a.C;
+  Pack<E, V> x[N];
+  gn_load<E, N, V>(static_cast<const E*>(a.x) + at, step, rows, x);
+  const int per_row = WHOLE ? a.cg / V : a.cg, parts = a.rpp * per_row;  // of one group
+  if (q.live) {
+    if (WHOLE) {
+      const int g = q.cv / a.cg;
+      part[g * parts + q.r * per_row + (q.cv - g * a.cg) / V] = gn_moments<E, N, V, V>(x, rows, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int g = (q.cv + j) / a.cg;
+        part[g * parts + q.r * per_row + (q.cv + j - g * a.cg)] = gn_moments<E, N, V, 1>(x, rows, j);
+      }
+    }
+  }
+  __syncthreads();
+  // one warp per group
   const int lane = threadIdx.x & 31;
-  const int64_t s = u / a.G, g = u - s * a.G, k = (int64_t)a.tiles * a.cg;
+  const float total = (float)a.P * (float)a.cg;
+  float2* const stat = reinterpret_cast<float2*>(part + a.k * parts);  // [k]
+  for (int g = threadIdx.x >> 5; g < ng; g += kGnThreads / 32) {
+    float sum = 0.0f, m2 = 0.0f;
+    for (int i = lane; i < parts; i += 32) {
+      const float4 v = part[g * parts + i];
+      sum = fmaf(v.z, v.x, sum);
+    }
+    const float mean = gn_warp_sum(sum) / total;
+    for (int i = lane; i < parts; i += 32) {
+      const float4 v = part[g * parts + i];
+      const float d = v.x - mean;
+      m2 += fmaf(v.z * d, d, v.y);
+    }
+    const float rstd = rsqrtf(gn_warp_sum(m2) / total + a.eps);
+    if (lane == 0) {
+      stat[g] = make_float2(mean, rstd);
+      if (a.mean != nullptr) {
+        a.mean[s * a.G + g0 + g] = mean;
+        a.rstd[s * a.G + g0 + g] = rstd;
+      }
+    }
+  }
+  __syncthreads();
+  if (!q.live) return;
+  GnAffine<V> f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float2 m = stat[WHOLE ? q.cv / a.cg : (q.cv + j) / a.cg];
+    f.mean[j] = m.x;
+    f.rstd[j] = m.y;
+    f.w[j] = a.weight != nullptr ? a.weight[c0 + j] : 1.0f;
+    f.b[j] = a.bias != nullptr ? a.bias[c0 + j] : 0.0f;
+  }
+  E* const y = static_cast<E*>(a.y) + at;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < rows) store_pack<E, V>(y + i * step, gn_forward<E, ACT, V>(x[i], f, a.thr));
+}
+
+// Sums over the rows of part [rpp][width], by the whole block and in a fixed
+// order: `some` [segments][width] (at most one entry per thread), then sums [width].
+__device__ __forceinline__ void gn_channel_sums(const float2* part, int rpp, int width, float2* some, float2* sums) {
+  const int segments = max(1, min(rpp, kGnThreads / width));
+  for (int i = threadIdx.x; i < segments * width; i += kGnThreads) {
+    const int seg = i / width, c = i - seg * width;
+    float2 v = make_float2(0.0f, 0.0f);
+    for (int r = seg; r < rpp; r += segments) {
+      v.x += part[r * width + c].x;
+      v.y += part[r * width + c].y;
+    }
+    (segments > 1 ? some : sums)[i] = v;
+  }
+  __syncthreads();
+  if (segments > 1) {
+    for (int c = threadIdx.x; c < width; c += kGnThreads) {
+      float2 v = some[c];
+      for (int i = 1; i < segments; ++i) {
+        v.x += some[i * width + c].x;
+        v.y += some[i * width + c].y;
+      }
+      sums[c] = v;
+    }
+    __syncthreads();
+  }
+}
+
+template <typename E, int ACT, int N>
+__global__ void __launch_bounds__(kGnThreads, 2) gn_resident_backward_kernel(GnArgs a) {
+  constexpr int V = 16 / (int)sizeof(E);
+  extern __shared__ __align__(16) unsigned char gn_smem[];
+  float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][width] sums of dz and dz xhat
+  const int64_t s = blockIdx.x / a.tiles;
+  const int g0 = (int)(blockIdx.x - s * a.tiles) * a.k, ng = min(a.k, a.G - g0), width = ng * a.cg;
+  GnSpot q = gn_spot(V, a.tpr, a.rpp);
+  q.live = q.live && q.cv < width;
+  const int rows = gn_rows<N>(a, q), c0 = g0 * a.cg + q.cv;
+  const int64_t at = (s * a.P + q.r) * a.C + c0, step = (int64_t)a.rpp * a.C;
+  Pack<E, V> x[N], gy[N];
+  gn_load<E, N, V>(static_cast<const E*>(a.x) + at, step, rows, x);
+  gn_load<E, N, V>(static_cast<const E*>(a.gy) + at, step, rows, gy);
+  GnAffine<V> f;
+  if (q.live) {
+    gn_affine<V>(a, s, c0, &f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < rows) {
+          float xhat;
+          const float dz = gn_dz<E, ACT, V>(x[i], gy[i], f, j, a.thr, &xhat);
+          acc.x += dz;
+          acc.y = fmaf(dz, xhat, acc.y);
+        }
+      part[q.r * width + q.cv + j] = acc;
+    }
+  }
+  __syncthreads();
+  float2* const sums = part + a.rpp * a.k * a.cg;  // [width]
+  float2* const coef = sums + a.k * a.cg;          // [k]
+  gn_channel_sums(part, a.rpp, width, coef + a.k, sums);
+  const int lane = threadIdx.x & 31;
+  const float inv = 1.0f / ((float)a.P * (float)a.cg);
+  for (int g = threadIdx.x >> 5; g < ng; g += kGnThreads / 32) {
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int i = lane; i < a.cg; i += 32) {
+      const float w = a.weight != nullptr ? a.weight[(g0 + g) * a.cg + i] : 1.0f;
+      s1 = fmaf(w, sums[g * a.cg + i].x, s1);
+      s2 = fmaf(w, sums[g * a.cg + i].y, s2);
+    }
+    s1 = gn_warp_sum(s1);
+    s2 = gn_warp_sum(s2);
+    if (lane == 0) coef[g] = make_float2(s1 * inv, s2 * inv);
+  }
+  if (a.part != nullptr)
+    for (int c = threadIdx.x; c < width; c += kGnThreads)
+      *reinterpret_cast<float2*>(a.part + (s * a.C + g0 * a.cg + c) * 2) = sums[c];
+  __syncthreads();
+  if (!q.live) return;
+  E* const dx = static_cast<E*>(a.y) + at;
+  float2 m[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) m[j] = coef[(q.cv + j) / a.cg];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i < rows) {
+      Pack<E, V> o;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float xhat;
+        const float dz = gn_dz<E, ACT, V>(x[i], gy[i], f, j, a.thr, &xhat);
+        o.e[j] = elem_from_f32<E>(f.rstd[j] * (fmaf(dz, f.w[j], -m[j].x) - xhat * m[j].y));
+      }
+      store_pack<E, V>(dx + i * step, o);
+    }
+  }
+}
+
+// ---- tiled form: samples larger than a block holds.  Tiles of `rows`
+// positions; a tile's moments (sums) per channel, the join per sample and
+// group, then the apply pass, whose tiles run from the last to the first, so
+// that it finds in L2 what the first pass read last.
+struct GnTile {
+  int64_t s, p0;
+  int rows, c0;  // positions, the thread's first channel
+  bool live;
+};
+
+template <int V>
+__device__ __forceinline__ GnTile gn_tile(const GnArgs& a, int64_t tile, const GnSpot& q) {
+  GnTile t;
+  t.s = tile / a.tiles;
+  t.p0 = (tile - t.s * a.tiles) * a.rows;
+  t.rows = (int)min64(a.rows, a.P - t.p0);
+  t.c0 = (int)blockIdx.y * a.tpr * V + q.cv;
+  t.live = q.live && t.c0 < a.C;
+  return t;
+}
+
+constexpr int kGnBatch = 4;  // rows in flight per thread
+
+template <typename E, int V>
+__global__ void __launch_bounds__(2 * kGnThreads) gn_stats_kernel(GnArgs a) {
+  extern __shared__ __align__(16) unsigned char gn_smem[];
+  float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][tpr V]
+  const GnSpot q = gn_spot(V, a.tpr, a.rpp);
+  const GnTile t = gn_tile<V>(a, blockIdx.x, q);
+  float mean[V], m2[V], n = 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.0f;
+  if (t.live) {
+    const E* x = static_cast<const E*>(a.x) + (t.s * a.P + t.p0) * a.C + t.c0;
+    for (int p = q.r; p < t.rows; p += kGnBatch * a.rpp) {
+      Pack<E, V> v[kGnBatch];
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kGnBatch; ++i)
+        if (p + i * a.rpp < t.rows) {
+          v[i] = load_pack<E, V>(x + (int64_t)(p + i * a.rpp) * a.C);
+          m += 1.0f;
+        }
+      const float inv = __fdividef(1.0f, m), w = __fdividef(m, n + m), nw = n * w;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kGnBatch; ++i)
+          if (p + i * a.rpp < t.rows) sum += elem_to_f32(v[i].e[j]);
+        const float mb = sum * inv, d = mb - mean[j];
+        m2[j] = fmaf(d * d, nw, m2[j]);
+#pragma unroll
+        for (int i = 0; i < kGnBatch; ++i)
+          if (p + i * a.rpp < t.rows) {
+            const float e = elem_to_f32(v[i].e[j]) - mb;
+            m2[j] = fmaf(e, e, m2[j]);
+          }
+        mean[j] = fmaf(d, w, mean[j]);
+      }
+      n += m;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[q.r * a.tpr * V + q.cv + j] = make_float2(mean[j], m2[j]);
+  }
+  __syncthreads();
+  // the row threads' parts of one channel, in a fixed order
+  const int width = min(a.tpr * V, a.C - (int)blockIdx.y * a.tpr * V);
+  for (int c = threadIdx.x; c < width; c += blockDim.x) {
+    float2 v = part[c];
+    float cnt = (float)(int)ceil_div(t.rows, a.rpp);
+    for (int r = 1; r < a.rpp && r < t.rows; ++r) {
+      const float2 o = part[r * a.tpr * V + c];
+      const float k = (float)(int)ceil_div(t.rows - r, a.rpp), w = __fdividef(k, cnt + k), d = o.x - v.x;
+      v.x = fmaf(d, w, v.x);
+      v.y += fmaf(d * d, cnt * w, o.y);
+      cnt += k;
+    }
+    *reinterpret_cast<float2*>(a.part + ((int64_t)blockIdx.x * a.C + blockIdx.y * a.tpr * V + c) * 2) = v;
+  }
+}
+
+template <int THREADS>
+__device__ __forceinline__ float gn_block_sum(float v, float* sm) {
+  v = gn_warp_sum(v);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float r = 0.0f;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) r += sm[i];
+  __syncthreads();
+  return r;
+}
+
+// One block per (sample, group): joins the tiles' moments.
+__global__ void __launch_bounds__(kGnThreads) gn_stats_finish_kernel(GnArgs a) {
+  __shared__ float sm[kGnThreads / 32];
+  const int64_t u = blockIdx.x, s = u / a.G, g = u - s * a.G;
+  const int64_t parts = (int64_t)a.tiles * a.cg;
+  const float2* part = reinterpret_cast<const float2*>(a.part) + s * a.tiles * a.C + g * a.cg;
   const float total = (float)a.P * (float)a.cg;
   float sum = 0.0f, m2 = 0.0f;
-  for (int64_t i = lane; i < k; i += 32) {
-    const int64_t t = i / a.cg, c = g * a.cg + (i - t * a.cg);
-    const float n = (float)(min64((t + 1) * a.rows, a.P) - t * a.rows);
-    sum = fmaf(n, a.part[((s * a.tiles + t) * a.C + c) * 2], sum);
+  for (int64_t i = threadIdx.x; i < parts; i += kGnThreads) {
+    const int t = (int)(i / a.cg);
+    const float n = (float)(int)min64(a.rows, a.P - (int64_t)t * a.rows);
+    sum = fmaf(n, part[(int64_t)t * a.C + (i - (int64_t)t * a.cg)].x, sum);
   }
-  const float mean = gn_warp_sum(sum) / total;
-  for (int64_t i = lane; i < k; i += 32) {
-    const int64_t t = i / a.cg, c = g * a.cg + (i - t * a.cg);
-    const float n = (float)(min64((t + 1) * a.rows, a.P) - t * a.rows);
-    const float* part = a.part + ((s * a.tiles + t) * a.C + c) * 2;
-    const float d = part[0] - mean;
-    m2 += fmaf(n * d, d, part[1]);
+  const float mean = gn_block_sum<kGnThreads>(sum, sm) / total;
+  for (int64_t i = threadIdx.x; i < parts; i += kGnThreads) {
+    const int t = (int)(i / a.cg);
+    const float n = (float)(int)min64(a.rows, a.P - (int64_t)t * a.rows);
+    const float2 v = part[(int64_t)t * a.C + (i - (int64_t)t * a.cg)];
+    const float d = v.x - mean;
+    m2 += fmaf(n * d, d, v.y);
   }
-  const float var = gn_warp_sum(m2) / total;
-  if (lane == 0) {
+  const float var = gn_block_sum<kGnThreads>(m2, sm) / total;
+  if (threadIdx.x == 0) {
     a.mean[u] = mean;
     a.rstd[u] = rsqrtf(var + a.eps);
   }
 }
 
-template <typename E, int ACT>
-__global__ void __launch_bounds__(kGnThreads) gn_apply_kernel(GnArgs a) {
-  const int64_t n = a.S * a.P * a.C, step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t row = i / a.C;
-    const int c = (int)(i - row * a.C);
-    const int64_t u = (row / a.P) * a.G + c / a.cg;
-    const float w = a.weight != nullptr ? a.weight[c] : 1.0f, b = a.bias != nullptr ? a.bias[c] : 0.0f;
-    const float xhat = (elem_to_f32(static_cast<const E*>(a.x)[i]) - a.mean[u]) * a.rstd[u];
-    static_cast<E*>(a.y)[i] = elem_from_f32<E>(gn_act<ACT>(fmaf(xhat, w, b), a.thr));
+template <typename E, int ACT, int V>
+__global__ void __launch_bounds__(2 * kGnThreads) gn_apply_kernel(GnArgs a) {
+  const GnSpot q = gn_spot(V, a.tpr, a.rpp);
+  const GnTile t = gn_tile<V>(a, gridDim.x - 1 - (int64_t)blockIdx.x, q);
+  if (!t.live) return;
+  GnAffine<V> f;
+  gn_affine<V>(a, t.s, t.c0, &f);
+  const int64_t at = (t.s * a.P + t.p0) * a.C + t.c0;
+  const E* x = static_cast<const E*>(a.x) + at;
+  E* y = static_cast<E*>(a.y) + at;
+  for (int p = q.r; p < t.rows; p += kGnBatch * a.rpp) {
+    Pack<E, V> v[kGnBatch];
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i)
+      if (p + i * a.rpp < t.rows) v[i] = load_pack<E, V>(x + (int64_t)(p + i * a.rpp) * a.C);
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i)
+      if (p + i * a.rpp < t.rows)
+        store_pack<E, V>(y + (int64_t)(p + i * a.rpp) * a.C, gn_forward<E, ACT, V>(v[i], f, a.thr));
   }
 }
 
 // Backward, per tile and channel: sum dz and sum dz xhat.
-template <typename E, int ACT>
-__global__ void __launch_bounds__(kGnThreads) gn_grad_sums_kernel(GnArgs a) {
-  __shared__ float2 sm[8][32];
-  const int c = blockIdx.y * 32 + threadIdx.x;
-  const int64_t tile = blockIdx.x, s = tile / a.tiles;
-  const int64_t p0 = (tile - s * a.tiles) * a.rows, p1 = min64(p0 + a.rows, a.P);
-  float2 acc = make_float2(0.0f, 0.0f);
-  if (c < a.C) {
-    const float w = a.weight != nullptr ? a.weight[c] : 1.0f, b = a.bias != nullptr ? a.bias[c] : 0.0f;
-    const float mean = a.mean[s * a.G + c / a.cg], rstd = a.rstd[s * a.G + c / a.cg];
-    for (int64_t p = p0 + threadIdx.y; p < p1; p += 8) {
-      const int64_t i = (s * a.P + p) * a.C + c;
-      const float xhat = (elem_to_f32(static_cast<const E*>(a.x)[i]) - mean) * rstd;
-      const float dz = gn_act_grad<ACT>(fmaf(xhat, w, b), a.thr, elem_to_f32(static_cast<const E*>(a.gy)[i]));
-      acc.x += dz;
-      acc.y = fmaf(dz, xhat, acc.y);
+template <typename E, int ACT, int V>
+__global__ void __launch_bounds__(2 * kGnThreads) gn_grad_sums_kernel(GnArgs a) {
+  extern __shared__ __align__(16) unsigned char gn_smem[];
+  float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][tpr V]
+  const GnSpot q = gn_spot(V, a.tpr, a.rpp);
+  const GnTile t = gn_tile<V>(a, blockIdx.x, q);
+  if (t.live) {
+    GnAffine<V> f;
+    gn_affine<V>(a, t.s, t.c0, &f);
+    const int64_t at = (t.s * a.P + t.p0) * a.C + t.c0;
+    const E *x = static_cast<const E*>(a.x) + at, *gy = static_cast<const E*>(a.gy) + at;
+    float2 acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = make_float2(0.0f, 0.0f);
+    for (int p = q.r; p < t.rows; p += kGnBatch * a.rpp) {
+      Pack<E, V> v[kGnBatch], d[kGnBatch];
+#pragma unroll
+      for (int i = 0; i < kGnBatch; ++i)
+        if (p + i * a.rpp < t.rows) {
+          v[i] = load_pack<E, V>(x + (int64_t)(p + i * a.rpp) * a.C);
+          d[i] = load_pack<E, V>(gy + (int64_t)(p + i * a.rpp) * a.C);
+        }
+#pragma unroll
+      for (int i = 0; i < kGnBatch; ++i)
+        if (p + i * a.rpp < t.rows) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            float xhat;
+            const float dz = gn_dz<E, ACT, V>(v[i], d[i], f, j, a.thr, &xhat);
+            acc[j].x += dz;
+            acc[j].y = fmaf(dz, xhat, acc[j].y);
+          }
+        }
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[q.r * a.tpr * V + q.cv + j] = acc[j];
   }
-  sm[threadIdx.y][threadIdx.x] = acc;
   __syncthreads();
-  if (threadIdx.y == 0 && c < a.C) {
-    for (int i = 1; i < 8; ++i) {
-      acc.x += sm[i][threadIdx.x].x;
-      acc.y += sm[i][threadIdx.x].y;
+  const int width = min(a.tpr * V, a.C - (int)blockIdx.y * a.tpr * V);
+  for (int c = threadIdx.x; c < width; c += blockDim.x) {
+    float2 v = part[c];
+    for (int r = 1; r < a.rpp; ++r) {
+      v.x += part[r * a.tpr * V + c].x;
+      v.y += part[r * a.tpr * V + c].y;
     }
-    *reinterpret_cast<float2*>(a.part + (tile * a.C + c) * 2) = acc;
+    *reinterpret_cast<float2*>(a.part + ((int64_t)blockIdx.x * a.C + blockIdx.y * a.tpr * V + c) * 2) = v;
   }
 }
 
-// One warp per (sample, group): mean(dn) and mean(dn xhat).
+// One block per (sample, group): mean(dn) and mean(dn xhat).
 __global__ void __launch_bounds__(kGnThreads) gn_grad_finish_kernel(GnArgs a) {
-  const int64_t u = (int64_t)blockIdx.x * (kGnThreads / 32) + (threadIdx.x >> 5);
-  if (u >= a.S * a.G) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t s = u / a.G, g = u - s * a.G, k = (int64_t)a.tiles * a.cg;
+  __shared__ float sm[kGnThreads / 32];
+  const int64_t u = blockIdx.x, s = u / a.G, g = u - s * a.G;
+  const int64_t parts = (int64_t)a.tiles * a.cg;
+  const float2* part = reinterpret_cast<const float2*>(a.part) + s * a.tiles * a.C + g * a.cg;
   float s1 = 0.0f, s2 = 0.0f;
-  for (int64_t i = lane; i < k; i += 32) {
-    const int64_t t = i / a.cg, c = g * a.cg + (i - t * a.cg);
-    const float w = a.weight != nullptr ? a.weight[c] : 1.0f;
-    const float* part = a.part + ((s * a.tiles + t) * a.C + c) * 2;
-    s1 = fmaf(w, part[0], s1);
-    s2 = fmaf(w, part[1], s2);
+  for (int64_t i = threadIdx.x; i < parts; i += kGnThreads) {
+    const int t = (int)(i / a.cg), c = (int)(i - (int64_t)t * a.cg);
+    const float w = a.weight != nullptr ? a.weight[g * a.cg + c] : 1.0f;
+    const float2 v = part[(int64_t)t * a.C + c];
+    s1 = fmaf(w, v.x, s1);
+    s2 = fmaf(w, v.y, s2);
   }
-  s1 = gn_warp_sum(s1);
-  s2 = gn_warp_sum(s2);
-  if (lane == 0) {
+  s1 = gn_block_sum<kGnThreads>(s1, sm);
+  s2 = gn_block_sum<kGnThreads>(s2, sm);
+  if (threadIdx.x == 0) {
     const float inv = 1.0f / ((float)a.P * (float)a.cg);
     a.coef[2 * u] = s1 * inv;
     a.coef[2 * u + 1] = s2 * inv;
   }
 }
 
-template <typename E, int ACT>
-__global__ void __launch_bounds__(kGnThreads) gn_grad_apply_kernel(GnArgs a) {
-  const int64_t n = a.S * a.P * a.C, step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t row = i / a.C;
-    const int c = (int)(i - row * a.C);
-    const int64_t u = (row / a.P) * a.G + c / a.cg;
-    const float w = a.weight != nullptr ? a.weight[c] : 1.0f, b = a.bias != nullptr ? a.bias[c] : 0.0f;
-    const float rstd = a.rstd[u];
-    const float xhat = (elem_to_f32(static_cast<const E*>(a.x)[i]) - a.mean[u]) * rstd;
-    const float dz = gn_act_grad<ACT>(fmaf(xhat, w, b), a.thr, elem_to_f32(static_cast<const E*>(a.gy)[i]));
-    static_cast<E*>(a.y)[i] = elem_from_f32<E>(rstd * (dz * w - a.coef[2 * u] - xhat * a.coef[2 * u + 1]));
+template <typename E, int ACT, int V>
+__global__ void __launch_bounds__(2 * kGnThreads) gn_grad_apply_kernel(GnArgs a) {
+  const GnSpot q = gn_spot(V, a.tpr, a.rpp);
+  const GnTile t = gn_tile<V>(a, gridDim.x - 1 - (int64_t)blockIdx.x, q);
+  if (!t.live) return;
+  GnAffine<V> f;
+  gn_affine<V>(a, t.s, t.c0, &f);
+  float2 m[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    m[j] = *reinterpret_cast<const float2*>(a.coef + 2 * (t.s * a.G + (t.c0 + j) / a.cg));
+  const int64_t at = (t.s * a.P + t.p0) * a.C + t.c0;
+  const E *x = static_cast<const E*>(a.x) + at, *gy = static_cast<const E*>(a.gy) + at;
+  E* dx = static_cast<E*>(a.y) + at;
+  for (int p = q.r; p < t.rows; p += kGnBatch * a.rpp) {
+    Pack<E, V> v[kGnBatch], d[kGnBatch];
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i)
+      if (p + i * a.rpp < t.rows) {
+        v[i] = load_pack<E, V>(x + (int64_t)(p + i * a.rpp) * a.C);
+        d[i] = load_pack<E, V>(gy + (int64_t)(p + i * a.rpp) * a.C);
+      }
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i)
+      if (p + i * a.rpp < t.rows) {
+        Pack<E, V> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float xhat;
+          const float dz = gn_dz<E, ACT, V>(v[i], d[i], f, j, a.thr, &xhat);
+          o.e[j] = elem_from_f32<E>(f.rstd[j] * (fmaf(dz, f.w[j], -m[j].x) - xhat * m[j].y));
+        }
+        store_pack<E, V>(dx + (int64_t)(p + i * a.rpp) * a.C, o);
+      }
   }
 }
 
@@ -221,8 +591,7 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(GnArgs a) {
   const int c = blockIdx.x * 32 + threadIdx.x;
   float2 acc = make_float2(0.0f, 0.0f);
   if (c < a.C) {
-    const int64_t rows = a.S * a.tiles;
-    for (int64_t r = threadIdx.y; r < rows; r += 32) {
+    for (int64_t r = threadIdx.y; r < a.parts; r += 32) {
       const float2 v = *reinterpret_cast<const float2*>(a.part + (r * a.C + c) * 2);
       acc.x += v.x;
       acc.y += v.y;
@@ -239,18 +608,82 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(GnArgs a) {
   }
 }
 
-// Positions per tile: enough tiles to fill the GPU, at least 64 positions each
-// so that the partial sums stay small beside the tensor.
-static void gn_tiling(int64_t S, int64_t P, int C, int* rows, int* tiles) {
-  const int64_t want = ceil_div(148 * 8, max64(S * ceil_div(C, 32), 1));
-  const int64_t r = max64(64, max64(ceil_div(P, max64(want, 1)), ceil_div(P, 65535)));
+// ---- plans
+static int64_t gn_gcd(int64_t a, int64_t b) { return b == 0 ? a : gn_gcd(b, a % b); }
+
+// Channels per thread: 16 bytes of them, else 2, else 1, as shape and pointers allow.
+static int gn_vector(size_t eb, int C, const void* x, const void* gy, const void* y) {
+  const int wide = 16 / (int)eb;
+  for (int v : {wide, 2}) {
+    const size_t bytes = v * eb;
+    if (C % v == 0 && aligned_to(x, bytes) && aligned_to(gy, bytes) && aligned_to(y, bytes)) return v;
+  }
+  return 1;
+}
+
+// Resident form: the largest k groups per block whose positions fit into N
+// packs per thread and that leave enough blocks for the GPU; rows of at least
+// 64 bytes.  False: none (the sample is too large, or its rows do not divide
+// into packs).
+static bool gn_resident_plan(GnArgs* a, size_t eb, int V, int N) {
+  if (V != 16 / (int)eb) return false;
+  const int64_t unit = V / gn_gcd(a->cg, V);  // groups that make whole packs
+  for (int64_t k = ceil_div(a->G, unit) * unit; k >= 1; k -= unit) {
+    const int64_t kk = k > a->G ? a->G : k, width = kk * a->cg;
+    if (kk < a->G && (int64_t)(width * eb) < 64) return false;
+    if (width / V > kGnThreads) continue;
+    const int tpr = (int)(width / V), rpp = kGnThreads / tpr;
+    if (ceil_div(a->P, rpp) > N) continue;
+    const int64_t smaller = kk > unit ? (kk - 1) / unit * unit : kk;
+    if (a->S * ceil_div(a->G, kk) < 2 * 148 && smaller < kk && (int64_t)(smaller * a->cg * eb) >= 64) continue;
+    a->k = (int)kk;
+    a->tpr = tpr;
+    a->rpp = rpp;
+    a->tiles = (int)ceil_div(a->G, kk);
+    a->parts = a->S;
+    return a->S * a->tiles < (1ll << 31);
+  }
+  return false;
+}
+
+static size_t gn_resident_smem(const GnArgs& a, int V, bool whole, bool backward) {
+  const size_t width = (size_t)a.k * a.cg;
+  if (backward) return (width * a.rpp + width + a.k + kGnThreads) * sizeof(float2);
+  return width / (whole ? V : 1) * a.rpp * sizeof(float4) + a.k * sizeof(float2);
+}
+
+// Tiled form: blocks of up to 512 threads whose rows waste the fewest of them,
+// tiles of at least 128 positions (the partial sums stay below a few percent
+// of the tensor) and enough of them for the GPU.
+static void gn_tiled_rows(int64_t S, int64_t P, int C, int* rows, int* tiles) {
+  const int64_t want = ceil_div(148 * 4, max64(S, 1));
+  const int64_t r = max64(128, max64(ceil_div(P, want), ceil_div(P, 65535)));
   *rows = (int)min64(r, max64(P, 1));
   *tiles = (int)ceil_div(max64(P, 1), *rows);
 }
 
+static void gn_tiled_plan(GnArgs* a, int V) {
+  const int per_row = (int)ceil_div(a->C, V);
+  a->tpr = per_row > 2 * kGnThreads ? kGnThreads : per_row;
+  a->rpp = 1;
+  a->threads = 32 * (int)ceil_div(a->tpr, 32);
+  double best = 0.0;
+  for (int rpp = 1; rpp * a->tpr <= 2 * kGnThreads && rpp <= 64; ++rpp) {
+    const int threads = 32 * (int)ceil_div(rpp * a->tpr, 32);
+    const double used = (double)(rpp * a->tpr) / threads * (threads >= 192 ? 1.0 : threads / 192.0);
+    if (used > best + 1e-9) {
+      best = used;
+      a->rpp = rpp;
+      a->threads = threads;
+    }
+  }
+  gn_tiled_rows(a->S, a->P, a->C, &a->rows, &a->tiles);
+  a->parts = a->S * a->tiles;
+}
+
 static size_t gn_part_bytes(int64_t S, int64_t P, int C) {
   int rows, tiles;
-  gn_tiling(S, P, C, &rows, &tiles);
+  gn_tiled_rows(S, P, C, &rows, &tiles);
   return align_up((size_t)S * tiles * C * 2 * sizeof(float), 256);
 }
 
@@ -262,12 +695,23 @@ static int gn_check(int dtype, int64_t S, int64_t P, int C, int G, int act, size
   SPK_REQUIRE(*eb != 0, "unknown element type %d", dtype);
   SPK_REQUIRE(act == SPK_ACT_NONE || act == SPK_ACT_HEAVISIDE || act == SPK_ACT_SILU,
               "unknown group norm activation %d", act);
-  SPK_REQUIRE(C <= (1 << 20) && P < (1ll << 31) && S < (1ll << 31) && (P == 0 || S < (1ll << 42) / ((int64_t)C * P)),
+  SPK_REQUIRE(C <= (1 << 20) && P < (1ll << 31) && S * G < (1ll << 31) && (P == 0 || S < (1ll << 42) / ((int64_t)C * P)),
               "shape too large (S=%lld, P=%lld, C=%d)", (long long)S, (long long)P, C);
   int rows, tiles;
-  gn_tiling(S, P, C, &rows, &tiles);
+  gn_tiled_rows(S, P, C, &rows, &tiles);
   SPK_REQUIRE(S * tiles < (1ll << 31), "too many positions (S=%lld, P=%lld)", (long long)S, (long long)P);
   return SPK_OK;
+}
+
+template <typename E, typename F>
+inline void with_gn_vector(int V, F&& f) {
+  constexpr int kWide = 16 / (int)sizeof(E);
+  if (V == kWide)
+    f(std::integral_constant<int, kWide>{});
+  else if (V == 2)
+    f(std::integral_constant<int, 2>{});
+  else
+    f(std::integral_constant<int, 1>{});
 }
 
 template <typename F>
@@ -319,17 +763,45 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
   a.cg = C / G;
   a.eps = eps;
   a.thr = thr;
-  spk::gn_tiling(S, P, C, &a.rows, &a.tiles);
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 tgrid((unsigned)(S * a.tiles), (unsigned)spk::ceil_div(C, 32)), tblock(32, 8);
-  const unsigned ugrid = (unsigned)spk::ceil_div(S * G, spk::kGnThreads / 32);
-  const unsigned egrid = (unsigned)spk::min64(spk::ceil_div(S * P * C, spk::kGnThreads), spk::sm_count() * 16);
+  const int V = spk::gn_vector(eb, C, X, nullptr, Y);
+  if (spk::gn_resident_plan(&a, eb, V, 16)) {
+    const bool whole = a.cg % V == 0;
+    const size_t smem = spk::gn_resident_smem(a, V, whole, false);
+    const bool few = spk::ceil_div(P, a.rpp) <= 4;
+    a.mean = mean;
+    a.rstd = rstd;
+    spk::with_elem(dtype, [&](auto e) {
+      using E = decltype(e);
+      spk::with_gn_act(act, [&](auto ac) {
+        constexpr int ACT = decltype(ac)::value;
+        const unsigned grid = (unsigned)(S * a.tiles);
+        if (few && whole)
+          spk::gn_resident_kernel<E, ACT, 4, true><<<grid, spk::kGnThreads, smem, st>>>(a);
+        else if (few)
+          spk::gn_resident_kernel<E, ACT, 4, false><<<grid, spk::kGnThreads, smem, st>>>(a);
+        else if (whole)
+          spk::gn_resident_kernel<E, ACT, 16, true><<<grid, spk::kGnThreads, smem, st>>>(a);
+        else
+          spk::gn_resident_kernel<E, ACT, 16, false><<<grid, spk::kGnThreads, smem, st>>>(a);
+      });
+    });
+    SPK_LAUNCH_CHECK();
+    spk::count_launch(1);
+    return SPK_OK;
+  }
+  spk::gn_tiled_plan(&a, V);
+  const dim3 grid((unsigned)a.parts, (unsigned)spk::ceil_div(C, a.tpr * V)), block((unsigned)a.threads);
+  const size_t smem = (size_t)a.rpp * a.tpr * V * sizeof(float2);
   spk::with_elem(dtype, [&](auto e) {
     using E = decltype(e);
-    spk::gn_stats_kernel<E><<<tgrid, tblock, 0, st>>>(a);
-    spk::gn_stats_finish_kernel<<<ugrid, spk::kGnThreads, 0, st>>>(a);
-    spk::with_gn_act(act, [&](auto ac) {
-      spk::gn_apply_kernel<E, decltype(ac)::value><<<egrid, spk::kGnThreads, 0, st>>>(a);
+    spk::with_gn_vector<E>(V, [&](auto vc) {
+      constexpr int VV = decltype(vc)::value;
+      spk::gn_stats_kernel<E, VV><<<grid, block, smem, st>>>(a);
+      spk::gn_stats_finish_kernel<<<(unsigned)(S * G), spk::kGnThreads, 0, st>>>(a);
+      spk::with_gn_act(act, [&](auto ac) {
+        spk::gn_apply_kernel<E, decltype(ac)::value, VV><<<grid, block, 0, st>>>(a);
+      });
     });
   });
   SPK_LAUNCH_CHECK();
@@ -379,21 +851,46 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
   a.G = G;
   a.cg = C / G;
   a.thr = thr;
-  spk::gn_tiling(S, P, C, &a.rows, &a.tiles);
-  const dim3 tgrid((unsigned)(S * a.tiles), (unsigned)spk::ceil_div(C, 32)), tblock(32, 8);
-  const unsigned ugrid = (unsigned)spk::ceil_div(S * G, spk::kGnThreads / 32);
-  const unsigned egrid = (unsigned)spk::min64(spk::ceil_div(S * P * C, spk::kGnThreads), spk::sm_count() * 16);
-  spk::with_elem(dtype, [&](auto e) {
-    using E = decltype(e);
-    spk::with_gn_act(act, [&](auto ac) {
-      constexpr int ACT = decltype(ac)::value;
-      spk::gn_grad_sums_kernel<E, ACT><<<tgrid, tblock, 0, st>>>(a);
-      spk::gn_grad_finish_kernel<<<ugrid, spk::kGnThreads, 0, st>>>(a);
-      spk::gn_grad_apply_kernel<E, ACT><<<egrid, spk::kGnThreads, 0, st>>>(a);
-      spk::gn_param_grad_kernel<<<(unsigned)spk::ceil_div(C, 32), dim3(32, 32), 0, st>>>(a);
+  const int V = spk::gn_vector(eb, C, X, GY, DX);
+  const bool params = dweight != nullptr || dbias != nullptr;
+  if (spk::gn_resident_plan(&a, eb, V, 8)) {
+    const size_t smem = spk::gn_resident_smem(a, V, false, true);
+    const bool few = spk::ceil_div(P, a.rpp) <= 4;
+    if (!params) a.part = nullptr;
+    spk::with_elem(dtype, [&](auto e) {
+      using E = decltype(e);
+      spk::with_gn_act(act, [&](auto ac) {
+        constexpr int ACT = decltype(ac)::value;
+        const unsigned grid = (unsigned)(S * a.tiles);
+        if (few)
+          spk::gn_resident_backward_kernel<E, ACT, 4><<<grid, spk::kGnThreads, smem, st>>>(a);
+        else
+          spk::gn_resident_backward_kernel<E, ACT, 8><<<grid, spk::kGnThreads, smem, st>>>(a);
+      });
     });
-  });
+    spk::count_launch(1);
+  } else {
+    spk::gn_tiled_plan(&a, V);
+    const dim3 grid((unsigned)a.parts, (unsigned)spk::ceil_div(C, a.tpr * V)), block((unsigned)a.threads);
+    const size_t smem = (size_t)a.rpp * a.tpr * V * sizeof(float2);
+    spk::with_elem(dtype, [&](auto e) {
+      using E = decltype(e);
+      spk::with_gn_vector<E>(V, [&](auto vc) {
+        constexpr int VV = decltype(vc)::value;
+        spk::with_gn_act(act, [&](auto ac) {
+          constexpr int ACT = decltype(ac)::value;
+          spk::gn_grad_sums_kernel<E, ACT, VV><<<grid, block, smem, st>>>(a);
+          spk::gn_grad_finish_kernel<<<(unsigned)(S * G), spk::kGnThreads, 0, st>>>(a);
+          spk::gn_grad_apply_kernel<E, ACT, VV><<<grid, block, 0, st>>>(a);
+        });
+      });
+    });
+    spk::count_launch(3);
+  }
+  if (params) {
+    spk::gn_param_grad_kernel<<<(unsigned)spk::ceil_div(C, 32), dim3(32, 32), 0, st>>>(a);
+    spk::count_launch(1);
+  }
   SPK_LAUNCH_CHECK();
-  spk::count_launch(4);
   return SPK_OK;
 }

@@ -95,17 +95,6 @@ struct GateForm {
   }
 };
 
-__device__ __forceinline__ float ex2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp_fast(float x) {  // a subnormal result becomes 0
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Leaky form, fp32 tensors.  A decay, of one step or of several, is whichever
 // of A and Q = 1 - A is at most one half, the sign bit set when it is A:
 // neither a slow channel's Q nor a fast channel's A is a difference from 1.
