@@ -87,40 +87,84 @@ __device__ __forceinline__ GnSpot gn_spot(int V, int tpr, int rpp) {
   return q;
 }
 
-// Per-channel constants of the thread's V channels.
-template <int V>
+// Constants of the thread's V channels, which lie in M groups at most (M = 1:
+// in one): with d = x - mean, z = d (rstd weight) + bias.
+template <int V, int M>
 struct GnAffine {
-  float mean[V], rstd[V], w[V], b[V];
+  float mean[M], rstd[M], a[V], b[V];
 };
 
-template <int V>
-__device__ __forceinline__ void gn_affine(const GnArgs& a, int64_t s, int c0, GnAffine<V>* f) {
+// f(j, group) for the channels c .. c + V - 1 of groups of cg channels.
+template <int V, int M, typename F>
+__device__ __forceinline__ void gn_groups(int c, int cg, F&& f) {
+  int g = c / cg, left = cg - (c - g * cg);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int64_t u = s * a.G + (c0 + j) / a.cg;
-    f->mean[j] = a.mean[u];
-    f->rstd[j] = a.rstd[u];
-    f->w[j] = a.weight != nullptr ? a.weight[c0 + j] : 1.0f;
+    if (M > 1 && left == 0) {
+      ++g;
+      left = cg;
+    }
+    f(j, g);
+    --left;
+  }
+}
+
+template <int V, int M>
+__device__ __forceinline__ void gn_affine(const GnArgs& a, int c0, GnAffine<V, M>* f) {  // mean and rstd are set
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    f->a[j] = f->rstd[M > 1 ? j : 0] * (a.weight != nullptr ? a.weight[c0 + j] : 1.0f);
     f->b[j] = a.bias != nullptr ? a.bias[c0 + j] : 0.0f;
   }
 }
 
-template <typename E, int ACT, int V>
-__device__ __forceinline__ Pack<E, V> gn_forward(const Pack<E, V>& x, const GnAffine<V>& f, float thr) {
+template <int V, int M>
+__device__ __forceinline__ void gn_affine(const GnArgs& a, int64_t s, int c0, GnAffine<V, M>* f) {
+  gn_groups<V, M>(c0, a.cg, [&](int j, int g) {
+    if (M > 1 || j == 0) {
+      f->mean[M > 1 ? j : 0] = a.mean[s * a.G + g];
+      f->rstd[M > 1 ? j : 0] = a.rstd[s * a.G + g];
+    }
+  });
+  gn_affine<V, M>(a, c0, f);
+}
+
+template <typename E, int ACT, int V, int M>
+__device__ __forceinline__ Pack<E, V> gn_forward(const Pack<E, V>& x, const GnAffine<V, M>& f, float thr) {
   Pack<E, V> y;
 #pragma unroll
   for (int j = 0; j < V; ++j)
     y.e[j] = elem_from_f32<E>(
-        gn_act<E, ACT>(fmaf((elem_to_f32(x.e[j]) - f.mean[j]) * f.rstd[j], f.w[j], f.b[j]), thr));
+        gn_act<E, ACT>(fmaf(elem_to_f32(x.e[j]) - f.mean[M > 1 ? j : 0], f.a[j], f.b[j]), thr));
   return y;
 }
 
-// dz and xhat of one element.
-template <typename E, int ACT, int V>
-__device__ __forceinline__ float gn_dz(const Pack<E, V>& x, const Pack<E, V>& gy, const GnAffine<V>& f, int j,
-                                       float thr, float* xhat) {
-  *xhat = (elem_to_f32(x.e[j]) - f.mean[j]) * f.rstd[j];
-  return gn_act_grad<E, ACT>(fmaf(*xhat, f.w[j], f.b[j]), thr, elem_to_f32(gy.e[j]));
+// dz and d of one element.
+template <typename E, int ACT, int V, int M>
+__device__ __forceinline__ float gn_dz(const Pack<E, V>& x, const Pack<E, V>& gy, const GnAffine<V, M>& f, int j,
+                                       float thr, float* d) {
+  *d = elem_to_f32(x.e[j]) - f.mean[M > 1 ? j : 0];
+  return gn_act_grad<E, ACT>(fmaf(*d, f.a[j], f.b[j]), thr, elem_to_f32(gy.e[j]));
+}
+
+// What a group's means m = (mean(dn), mean(dn xhat)) do to dx:
+// dx = rstd (dn - m.x - xhat m.y) = dz (rstd weight) + d k.y + k.x.
+__device__ __forceinline__ float2 gn_pull(float2 m, float rstd) {
+  return make_float2(-rstd * m.x, -rstd * rstd * m.y);
+}
+
+template <typename E, int ACT, int V, int M>
+__device__ __forceinline__ Pack<E, V> gn_backward(const Pack<E, V>& x, const Pack<E, V>& gy,
+                                                  const GnAffine<V, M>& f, const float2 (&k)[M], float thr) {
+  Pack<E, V> o;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    float d;
+    const float dz = gn_dz<E, ACT, V, M>(x, gy, f, j, thr, &d);
+    const float2 kj = k[M > 1 ? j : 0];
+    o.e[j] = elem_from_f32<E>(fmaf(dz, f.a[j], fmaf(d, kj.y, kj.x)));
+  }
+  return o;
 }
 
 // ---- resident form: a block holds a sample's k groups (all positions) in
@@ -163,8 +207,8 @@ __device__ __forceinline__ float4 gn_moments(const Pack<E, V>* x, int rows, int 
 
 // WHOLE: every pack lies in one group (cg is a multiple of V).
 template <typename E, int ACT, int N, bool WHOLE>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_resident_kernel(GnArgs a) {
-  constexpr int V = 16 / (int)sizeof(E);
+__global__ void __launch_bounds__(kGnThreads, N > 4 ? 2 : 4) gn_resident_kernel(GnArgs a) {
+  constexpr int V = 16 / (int)sizeof(E), M = WHOLE ? 1 : V;
   extern __shared__ __align__(16) unsigned char gn_smem[];
   float4* const part = reinterpret_cast<float4*>(gn_smem);  // [groups][parts] mean, sum of squares about it, count
   const int64_t s = blockIdx.x / a.tiles;
@@ -216,19 +260,18 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_resident_kernel(GnArgs a) {
   }
   __syncthreads();
   if (!q.live) return;
-  GnAffine<V> f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float2 m = stat[WHOLE ? q.cv / a.cg : (q.cv + j) / a.cg];
-    f.mean[j] = m.x;
-    f.rstd[j] = m.y;
-    f.w[j] = a.weight != nullptr ? a.weight[c0 + j] : 1.0f;
-    f.b[j] = a.bias != nullptr ? a.bias[c0 + j] : 0.0f;
-  }
+  GnAffine<V, M> f;
+  gn_groups<V, M>(q.cv, a.cg, [&](int j, int g) {
+    if (M > 1 || j == 0) {
+      f.mean[M > 1 ? j : 0] = stat[g].x;
+      f.rstd[M > 1 ? j : 0] = stat[g].y;
+    }
+  });
+  gn_affine<V, M>(a, c0, &f);
   E* const y = static_cast<E*>(a.y) + at;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (i < rows) store_pack<E, V>(y + i * step, gn_forward<E, ACT, V>(x[i], f, a.thr));
+    if (i < rows) store_pack<E, V>(y + i * step, gn_forward<E, ACT, V, M>(x[i], f, a.thr));
 }
 
 // Sums over the rows of part [rpp][width], by the whole block and in a fixed
@@ -258,9 +301,9 @@ __device__ __forceinline__ void gn_channel_sums(const float2* part, int rpp, int
   }
 }
 
-template <typename E, int ACT, int N>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_resident_backward_kernel(GnArgs a) {
-  constexpr int V = 16 / (int)sizeof(E);
+template <typename E, int ACT, int N, bool WHOLE>
+__global__ void __launch_bounds__(kGnThreads, N > 2 ? 2 : 3) gn_resident_backward_kernel(GnArgs a) {
+  constexpr int V = 16 / (int)sizeof(E), M = WHOLE ? 1 : V;
   extern __shared__ __align__(16) unsigned char gn_smem[];
   float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][width] sums of dz and dz xhat
   const int64_t s = blockIdx.x / a.tiles;
@@ -272,21 +315,27 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_resident_backward_kernel(GnA
   Pack<E, V> x[N], gy[N];
   gn_load<E, N, V>(static_cast<const E*>(a.x) + at, step, rows, x);
   gn_load<E, N, V>(static_cast<const E*>(a.gy) + at, step, rows, gy);
-  GnAffine<V> f;
+  GnAffine<V, M> f;
+  constexpr bool kKeep = N <= 2;  // dz and x - mean stay in registers; with more rows they are computed again
+  float keep_dz[kKeep ? N : 1][V], keep_d[kKeep ? N : 1][V];
   if (q.live) {
-    gn_affine<V>(a, s, c0, &f);
+    gn_affine<V, M>(a, s, c0, &f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (i < rows) {
-          float xhat;
-          const float dz = gn_dz<E, ACT, V>(x[i], gy[i], f, j, a.thr, &xhat);
+          float d;
+          const float dz = gn_dz<E, ACT, V, M>(x[i], gy[i], f, j, a.thr, &d);
+          if (kKeep) {
+            keep_dz[kKeep ? i : 0][j] = dz;
+            keep_d[kKeep ? i : 0][j] = d;
+          }
           acc.x += dz;
-          acc.y = fmaf(dz, xhat, acc.y);
+          acc.y = fmaf(dz, d, acc.y);
         }
-      part[q.r * width + q.cv + j] = acc;
+      part[q.r * width + q.cv + j] = make_float2(acc.x, acc.y * f.rstd[M > 1 ? j : 0]);
     }
   }
   __syncthreads();
@@ -312,22 +361,26 @@ __global__ void __launch_bounds__(kGnThreads, 2) gn_resident_backward_kernel(GnA
   __syncthreads();
   if (!q.live) return;
   E* const dx = static_cast<E*>(a.y) + at;
-  float2 m[V];
+  float2 k[M];
+  gn_groups<V, M>(q.cv, a.cg, [&](int j, int g) {
+    if (M > 1 || j == 0) k[M > 1 ? j : 0] = gn_pull(coef[g], f.rstd[M > 1 ? j : 0]);
+  });
 #pragma unroll
-  for (int j = 0; j < V; ++j) m[j] = coef[(q.cv + j) / a.cg];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < N; ++i)
     if (i < rows) {
-      Pack<E, V> o;
+      if (kKeep) {
+        Pack<E, V> o;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float xhat;
-        const float dz = gn_dz<E, ACT, V>(x[i], gy[i], f, j, a.thr, &xhat);
-        o.e[j] = elem_from_f32<E>(f.rstd[j] * (fmaf(dz, f.w[j], -m[j].x) - xhat * m[j].y));
+        for (int j = 0; j < V; ++j) {
+          const float2 kj = k[M > 1 ? j : 0];
+          o.e[j] = elem_from_f32<E>(
+              fmaf(keep_dz[kKeep ? i : 0][j], f.a[j], fmaf(keep_d[kKeep ? i : 0][j], kj.y, kj.x)));
+        }
+        store_pack<E, V>(dx + i * step, o);
+      } else {
+        store_pack<E, V>(dx + i * step, gn_backward<E, ACT, V, M>(x[i], gy[i], f, k, a.thr));
       }
-      store_pack<E, V>(dx + i * step, o);
     }
-  }
 }
 
 // ---- tiled form: samples larger than a block holds.  Tiles of `rows`
@@ -351,10 +404,10 @@ __device__ __forceinline__ GnTile gn_tile(const GnArgs& a, int64_t tile, const G
   return t;
 }
 
-constexpr int kGnBatch = 4;  // rows in flight per thread
+constexpr int kGnBatch = 4, kGnGradBatch = 2;  // rows in flight per thread (of one tensor, of two)
 
 template <typename E, int V>
-__global__ void __launch_bounds__(2 * kGnThreads) gn_stats_kernel(GnArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 4) gn_stats_kernel(GnArgs a) {
   extern __shared__ __align__(16) unsigned char gn_smem[];
   float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][tpr V]
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
@@ -452,13 +505,13 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_finish_kernel(GnArgs a) {
   }
 }
 
-template <typename E, int ACT, int V>
-__global__ void __launch_bounds__(2 * kGnThreads) gn_apply_kernel(GnArgs a) {
+template <typename E, int ACT, int V, int M>
+__global__ void __launch_bounds__(kGnThreads, 4) gn_apply_kernel(GnArgs a) {
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
   const GnTile t = gn_tile<V>(a, gridDim.x - 1 - (int64_t)blockIdx.x, q);
   if (!t.live) return;
-  GnAffine<V> f;
-  gn_affine<V>(a, t.s, t.c0, &f);
+  GnAffine<V, M> f;
+  gn_affine<V, M>(a, t.s, t.c0, &f);
   const int64_t at = (t.s * a.P + t.p0) * a.C + t.c0;
   const E* x = static_cast<const E*>(a.x) + at;
   E* y = static_cast<E*>(a.y) + at;
@@ -470,47 +523,47 @@ __global__ void __launch_bounds__(2 * kGnThreads) gn_apply_kernel(GnArgs a) {
 #pragma unroll
     for (int i = 0; i < kGnBatch; ++i)
       if (p + i * a.rpp < t.rows)
-        store_pack<E, V>(y + (int64_t)(p + i * a.rpp) * a.C, gn_forward<E, ACT, V>(v[i], f, a.thr));
+        store_pack<E, V>(y + (int64_t)(p + i * a.rpp) * a.C, gn_forward<E, ACT, V, M>(v[i], f, a.thr));
   }
 }
 
 // Backward, per tile and channel: sum dz and sum dz xhat.
-template <typename E, int ACT, int V>
-__global__ void __launch_bounds__(2 * kGnThreads) gn_grad_sums_kernel(GnArgs a) {
+template <typename E, int ACT, int V, int M>
+__global__ void __launch_bounds__(kGnThreads, 3) gn_grad_sums_kernel(GnArgs a) {
   extern __shared__ __align__(16) unsigned char gn_smem[];
   float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][tpr V]
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
   const GnTile t = gn_tile<V>(a, blockIdx.x, q);
   if (t.live) {
-    GnAffine<V> f;
-    gn_affine<V>(a, t.s, t.c0, &f);
+    GnAffine<V, M> f;
+    gn_affine<V, M>(a, t.s, t.c0, &f);
     const int64_t at = (t.s * a.P + t.p0) * a.C + t.c0;
     const E *x = static_cast<const E*>(a.x) + at, *gy = static_cast<const E*>(a.gy) + at;
     float2 acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = make_float2(0.0f, 0.0f);
-    for (int p = q.r; p < t.rows; p += kGnBatch * a.rpp) {
-      Pack<E, V> v[kGnBatch], d[kGnBatch];
+    for (int p = q.r; p < t.rows; p += kGnGradBatch * a.rpp) {
+      Pack<E, V> v[kGnGradBatch], d[kGnGradBatch];
 #pragma unroll
-      for (int i = 0; i < kGnBatch; ++i)
+      for (int i = 0; i < kGnGradBatch; ++i)
         if (p + i * a.rpp < t.rows) {
           v[i] = load_pack<E, V>(x + (int64_t)(p + i * a.rpp) * a.C);
           d[i] = load_pack<E, V>(gy + (int64_t)(p + i * a.rpp) * a.C);
         }
 #pragma unroll
-      for (int i = 0; i < kGnBatch; ++i)
+      for (int i = 0; i < kGnGradBatch; ++i)
         if (p + i * a.rpp < t.rows) {
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            float xhat;
-            const float dz = gn_dz<E, ACT, V>(v[i], d[i], f, j, a.thr, &xhat);
+            float xc;
+            const float dz = gn_dz<E, ACT, V, M>(v[i], d[i], f, j, a.thr, &xc);
             acc[j].x += dz;
-            acc[j].y = fmaf(dz, xhat, acc[j].y);
+            acc[j].y = fmaf(dz, xc, acc[j].y);
           }
         }
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) part[q.r * a.tpr * V + q.cv + j] = acc[j];
+    for (int j = 0; j < V; ++j) part[q.r * a.tpr * V + q.cv + j] = make_float2(acc[j].x, acc[j].y * f.rstd[M > 1 ? j : 0]);
   }
   __syncthreads();
   const int width = min(a.tpr * V, a.C - (int)blockIdx.y * a.tpr * V);
@@ -547,40 +600,34 @@ __global__ void __launch_bounds__(kGnThreads) gn_grad_finish_kernel(GnArgs a) {
   }
 }
 
-template <typename E, int ACT, int V>
-__global__ void __launch_bounds__(2 * kGnThreads) gn_grad_apply_kernel(GnArgs a) {
+template <typename E, int ACT, int V, int M>
+__global__ void __launch_bounds__(kGnThreads, 3) gn_grad_apply_kernel(GnArgs a) {
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
   const GnTile t = gn_tile<V>(a, gridDim.x - 1 - (int64_t)blockIdx.x, q);
   if (!t.live) return;
-  GnAffine<V> f;
-  gn_affine<V>(a, t.s, t.c0, &f);
-  float2 m[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    m[j] = *reinterpret_cast<const float2*>(a.coef + 2 * (t.s * a.G + (t.c0 + j) / a.cg));
+  GnAffine<V, M> f;
+  gn_affine<V, M>(a, t.s, t.c0, &f);
+  float2 k[M];
+  gn_groups<V, M>(t.c0, a.cg, [&](int j, int g) {
+    if (M > 1 || j == 0)
+      k[M > 1 ? j : 0] =
+          gn_pull(*reinterpret_cast<const float2*>(a.coef + 2 * (t.s * a.G + g)), f.rstd[M > 1 ? j : 0]);
+  });
   const int64_t at = (t.s * a.P + t.p0) * a.C + t.c0;
   const E *x = static_cast<const E*>(a.x) + at, *gy = static_cast<const E*>(a.gy) + at;
   E* dx = static_cast<E*>(a.y) + at;
-  for (int p = q.r; p < t.rows; p += kGnBatch * a.rpp) {
-    Pack<E, V> v[kGnBatch], d[kGnBatch];
+  for (int p = q.r; p < t.rows; p += kGnGradBatch * a.rpp) {
+    Pack<E, V> v[kGnGradBatch], d[kGnGradBatch];
 #pragma unroll
-    for (int i = 0; i < kGnBatch; ++i)
+    for (int i = 0; i < kGnGradBatch; ++i)
       if (p + i * a.rpp < t.rows) {
         v[i] = load_pack<E, V>(x + (int64_t)(p + i * a.rpp) * a.C);
         d[i] = load_pack<E, V>(gy + (int64_t)(p + i * a.rpp) * a.C);
       }
 #pragma unroll
-    for (int i = 0; i < kGnBatch; ++i)
-      if (p + i * a.rpp < t.rows) {
-        Pack<E, V> o;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float xhat;
-          const float dz = gn_dz<E, ACT, V>(v[i], d[i], f, j, a.thr, &xhat);
-          o.e[j] = elem_from_f32<E>(f.rstd[j] * (fmaf(dz, f.w[j], -m[j].x) - xhat * m[j].y));
-        }
-        store_pack<E, V>(dx + (int64_t)(p + i * a.rpp) * a.C, o);
-      }
+    for (int i = 0; i < kGnGradBatch; ++i)
+      if (p + i * a.rpp < t.rows)
+        store_pack<E, V>(dx + (int64_t)(p + i * a.rpp) * a.C, gn_backward<E, ACT, V, M>(v[i], d[i], f, k, a.thr));
   }
 }
 
@@ -652,23 +699,23 @@ static size_t gn_resident_smem(const GnArgs& a, int V, bool whole, bool backward
   return width / (whole ? V : 1) * a.rpp * sizeof(float4) + a.k * sizeof(float2);
 }
 
-// Tiled form: blocks of up to 512 threads whose rows waste the fewest of them,
-// tiles of at least 128 positions (the partial sums stay below a few percent
-// of the tensor) and enough of them for the GPU.
+// Tiled form: blocks of up to 256 threads whose rows waste the fewest of them,
+// tiles of at least 32 positions (the partial sums stay well below the tensor)
+// and enough of them for the GPU.
 static void gn_tiled_rows(int64_t S, int64_t P, int C, int* rows, int* tiles) {
   const int64_t want = ceil_div(148 * 4, max64(S, 1));
-  const int64_t r = max64(128, max64(ceil_div(P, want), ceil_div(P, 65535)));
+  const int64_t r = max64(32, max64(ceil_div(P, want), ceil_div(P, 65535)));
   *rows = (int)min64(r, max64(P, 1));
   *tiles = (int)ceil_div(max64(P, 1), *rows);
 }
 
 static void gn_tiled_plan(GnArgs* a, int V) {
   const int per_row = (int)ceil_div(a->C, V);
-  a->tpr = per_row > 2 * kGnThreads ? kGnThreads : per_row;
+  a->tpr = per_row > kGnThreads ? kGnThreads : per_row;
   a->rpp = 1;
   a->threads = 32 * (int)ceil_div(a->tpr, 32);
   double best = 0.0;
-  for (int rpp = 1; rpp * a->tpr <= 2 * kGnThreads && rpp <= 64; ++rpp) {
+  for (int rpp = 1; rpp * a->tpr <= kGnThreads && rpp <= 64; ++rpp) {
     const int threads = 32 * (int)ceil_div(rpp * a->tpr, 32);
     const double used = (double)(rpp * a->tpr) / threads * (threads >= 192 ? 1.0 : threads / 192.0);
     if (used > best + 1e-9) {
@@ -703,15 +750,18 @@ static int gn_check(int dtype, int64_t S, int64_t P, int C, int G, int act, size
   return SPK_OK;
 }
 
+// f(channels per thread, groups among them at most)
 template <typename E, typename F>
-inline void with_gn_vector(int V, F&& f) {
+inline void with_gn_vector(int V, int cg, F&& f) {
   constexpr int kWide = 16 / (int)sizeof(E);
-  if (V == kWide)
-    f(std::integral_constant<int, kWide>{});
+  if (V == kWide && cg % kWide == 0)
+    f(std::integral_constant<int, kWide>{}, std::integral_constant<int, 1>{});
+  else if (V == kWide)
+    f(std::integral_constant<int, kWide>{}, std::integral_constant<int, kWide>{});
   else if (V == 2)
-    f(std::integral_constant<int, 2>{});
+    f(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
   else
-    f(std::integral_constant<int, 1>{});
+    f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
 }
 
 template <typename F>
@@ -765,7 +815,7 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
   a.thr = thr;
   cudaStream_t st = (cudaStream_t)stream;
   const int V = spk::gn_vector(eb, C, X, nullptr, Y);
-  if (spk::gn_resident_plan(&a, eb, V, 16)) {
+  if (spk::gn_resident_plan(&a, eb, V, 4) || spk::gn_resident_plan(&a, eb, V, 16)) {
     const bool whole = a.cg % V == 0;
     const size_t smem = spk::gn_resident_smem(a, V, whole, false);
     const bool few = spk::ceil_div(P, a.rpp) <= 4;
@@ -795,12 +845,12 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
   const size_t smem = (size_t)a.rpp * a.tpr * V * sizeof(float2);
   spk::with_elem(dtype, [&](auto e) {
     using E = decltype(e);
-    spk::with_gn_vector<E>(V, [&](auto vc) {
-      constexpr int VV = decltype(vc)::value;
+    spk::with_gn_vector<E>(V, a.cg, [&](auto vc, auto mc) {
+      constexpr int VV = decltype(vc)::value, MM = decltype(mc)::value;
       spk::gn_stats_kernel<E, VV><<<grid, block, smem, st>>>(a);
       spk::gn_stats_finish_kernel<<<(unsigned)(S * G), spk::kGnThreads, 0, st>>>(a);
       spk::with_gn_act(act, [&](auto ac) {
-        spk::gn_apply_kernel<E, decltype(ac)::value, VV><<<grid, block, 0, st>>>(a);
+        spk::gn_apply_kernel<E, decltype(ac)::value, VV, MM><<<grid, block, 0, st>>>(a);
       });
     });
   });
@@ -853,19 +903,24 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
   a.thr = thr;
   const int V = spk::gn_vector(eb, C, X, GY, DX);
   const bool params = dweight != nullptr || dbias != nullptr;
-  if (spk::gn_resident_plan(&a, eb, V, 8)) {
+  if (spk::gn_resident_plan(&a, eb, V, 2) || spk::gn_resident_plan(&a, eb, V, 8)) {
     const size_t smem = spk::gn_resident_smem(a, V, false, true);
-    const bool few = spk::ceil_div(P, a.rpp) <= 4;
+    const bool whole = a.cg % V == 0;
+    const bool few = spk::ceil_div(P, a.rpp) <= 2;
     if (!params) a.part = nullptr;
     spk::with_elem(dtype, [&](auto e) {
       using E = decltype(e);
       spk::with_gn_act(act, [&](auto ac) {
         constexpr int ACT = decltype(ac)::value;
         const unsigned grid = (unsigned)(S * a.tiles);
-        if (few)
-          spk::gn_resident_backward_kernel<E, ACT, 4><<<grid, spk::kGnThreads, smem, st>>>(a);
+        if (few && whole)
+          spk::gn_resident_backward_kernel<E, ACT, 2, true><<<grid, spk::kGnThreads, smem, st>>>(a);
+        else if (few)
+          spk::gn_resident_backward_kernel<E, ACT, 2, false><<<grid, spk::kGnThreads, smem, st>>>(a);
+        else if (whole)
+          spk::gn_resident_backward_kernel<E, ACT, 8, true><<<grid, spk::kGnThreads, smem, st>>>(a);
         else
-          spk::gn_resident_backward_kernel<E, ACT, 8><<<grid, spk::kGnThreads, smem, st>>>(a);
+          spk::gn_resident_backward_kernel<E, ACT, 8, false><<<grid, spk::kGnThreads, smem, st>>>(a);
       });
     });
     spk::count_launch(1);
@@ -875,13 +930,13 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
     const size_t smem = (size_t)a.rpp * a.tpr * V * sizeof(float2);
     spk::with_elem(dtype, [&](auto e) {
       using E = decltype(e);
-      spk::with_gn_vector<E>(V, [&](auto vc) {
-        constexpr int VV = decltype(vc)::value;
+      spk::with_gn_vector<E>(V, a.cg, [&](auto vc, auto mc) {
+        constexpr int VV = decltype(vc)::value, MM = decltype(mc)::value;
         spk::with_gn_act(act, [&](auto ac) {
           constexpr int ACT = decltype(ac)::value;
-          spk::gn_grad_sums_kernel<E, ACT, VV><<<grid, block, smem, st>>>(a);
+          spk::gn_grad_sums_kernel<E, ACT, VV, MM><<<grid, block, smem, st>>>(a);
           spk::gn_grad_finish_kernel<<<(unsigned)(S * G), spk::kGnThreads, 0, st>>>(a);
-          spk::gn_grad_apply_kernel<E, ACT, VV><<<grid, block, 0, st>>>(a);
+          spk::gn_grad_apply_kernel<E, ACT, VV, MM><<<grid, block, 0, st>>>(a);
         });
       });
     });
