@@ -582,35 +582,52 @@ def temporal_mean(x):
 _DTYPES = {torch.float32: _lib.SPK_F32, torch.bfloat16: _lib.SPK_BF16, torch.float16: _lib.SPK_F16}
 
 
-def _dtype(t, what):
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise EngineError(f"{what}: float32, bfloat16 or float16 tensors required, got {t.dtype}") from None
-
-
-def _same_device(t, *others, what):
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise EngineError(f"{what}: tensors on {t.device} and {o.device}")
+def _checked(what, x, *others):
+    """The dtype code of x, a CUDA tensor of one of the three types; the others
+    (or None) on its device."""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda):
+        require_cuda(x, what=what)
+    dev = x.get_device()
+    for t in others:
+        if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == dev):
+            require_cuda(t, what=what)
+            raise EngineError(f"{what}: tensors on {x.device} and {t.device}")
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        raise EngineError(f"{what}: float32, bfloat16 or float16 tensors required, got {x.dtype}")
+    return code
 
 
 def _call(t, name, *args):
     """Entry point `name` on t's device and its current stream (the last argument)."""
     fn = getattr(_lib.load(), name)
-    if t.device.index == torch.cuda.current_device():
-        check(fn(*args, stream_of(t)), name)
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(t.device):
-            check(fn(*args, stream_of(t)), name)
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, name)
 
 
 def _scratch(t, nbytes):
-    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+    return t.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _backward(fn):
+    """A Function's backward made of engine calls, which have no backward of
+    their own: differentiating it again raises (and only then costs the wrapper)."""
+    guarded = torch.autograd.function.once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return staticmethod(backward)
 
 
 # ------------------------------------------------------------- gated linear recurrence
@@ -628,23 +645,25 @@ def _time_strides(t, dim):
     """(stride of the flattened batch, stride of time) of t with time at
     dimension `dim` and every other dimension but the last one batch; None when
     the batch dimensions do not flatten or the last one is not contiguous."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape, strides = t.shape, t.stride()
+    if shape[-1] > 1 and strides[-1] != 1:
         return None
     step, size = None, 1
-    for i in range(t.dim() - 2, -1, -1):  # from the innermost batch dimension outwards
-        if i == dim or t.shape[i] == 1:
+    for i in range(len(shape) - 2, -1, -1):  # from the innermost batch dimension outwards
+        n = shape[i]
+        if i == dim or n == 1:
             continue
         if step is None:
-            step, size = t.stride(i), t.shape[i]
-        elif t.stride(i) != step * size:
+            step, size = strides[i], n
+        elif strides[i] != step * size:
             return None
         else:
-            size *= t.shape[i]
-    return (step if step is not None else 0), t.stride(dim)
+            size *= n
+    return (step if step is not None else 0), strides[dim]
 
 
 def _time_major(t, dim):
-    """t itself, or a copy, such that _time_strides(result, dim') holds, and dim'."""
+    """t itself, or a copy whose batch dimensions flatten, and its _time_strides."""
     st = _time_strides(t, dim)
     if st is not None:
         return t, st
@@ -654,7 +673,7 @@ def _time_major(t, dim):
 
 def _empty_time(t, dim):
     """An uninitialised tensor of t's shape whose batch dimensions flatten, and its strides."""
-    out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    out = torch.empty_like(t, memory_format=torch.contiguous_format)
     return _time_major(out, dim) if out.numel() else (out, (0, 0))
 
 
@@ -669,7 +688,7 @@ def _recurrence_forward(x, gate, state, form, dim, lengths, keep):
     if keep:
         chunk = int(lib.spk_recurrence_chunk(_DTYPES[x.dtype], B, L, D))
         if L > chunk:
-            carry = torch.empty((L + chunk - 1) // chunk - 1, B, D, dtype=torch.float32, device=x.device)
+            carry = x.new_empty((L + chunk - 1) // chunk - 1, B, D, dtype=torch.float32)
     _call(x, "spk_recurrence", ptr(x), xb, xt, ptr(gate), gb, gt, _DTYPES[x.dtype], form, B, L, D, ptr(state),
           ptr(lengths), ptr(h), hb, ht, ptr(last), ptr(carry))
     return h, last, carry
@@ -684,8 +703,7 @@ class _GatedRecurrence(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return h, last
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, gh, glast):
         x, gate, state, lengths, carry = ctx.saved_tensors
         if gh is None and glast is None:
@@ -722,10 +740,8 @@ def gated_recurrence(x, gate, state=None, form="leaky", dim=-2, lengths=None):
     stays.  x and gate may be slices or broadcast views whose last dimension is
     contiguous.  Differentiable in x, gate and state."""
     what = "gated_recurrence"
-    require_cuda(x, gate, state, lengths, what=what)
+    _checked(what, x, gate, state, lengths)
     form = _form(form, what)
-    _dtype(x, what)
-    _same_device(x, gate, state, lengths, what=what)
     if gate.dtype != x.dtype or gate.shape != x.shape:
         raise EngineError(f"{what}: gate must have x's shape and dtype ({tuple(x.shape)}, {x.dtype}), "
                           f"got {tuple(gate.shape)}, {gate.dtype}")
@@ -734,7 +750,7 @@ def gated_recurrence(x, gate, state=None, form="leaky", dim=-2, lengths=None):
     dim %= x.dim()
     shape = x.shape[:dim] + x.shape[dim + 1:]
     if state is None:
-        state = torch.zeros(shape, dtype=torch.float32, device=x.device)
+        state = x.new_zeros(shape, dtype=torch.float32)
     elif state.dtype != torch.float32 or state.shape != shape:
         raise EngineError(f"{what}: state must be float32 of shape {tuple(shape)}, got {tuple(state.shape)}, "
                           f"{state.dtype}")
@@ -758,10 +774,8 @@ def gated_recurrence_step(x, gate, state, form="leaky", new_state=None):
     (contiguous float32; `state` itself updates it in place).  Not
     differentiable."""
     what = "gated_recurrence_step"
-    require_cuda(x, gate, state, new_state, what=what)
+    dt = _checked(what, x, gate, state, new_state)
     form = _form(form, what)
-    dt = _dtype(x, what)
-    _same_device(x, gate, state, new_state, what=what)
     if gate.dtype != x.dtype or gate.shape != x.shape:
         raise EngineError(f"{what}: gate must have x's shape and dtype")
     if state.dtype != torch.float32 or state.shape != x.shape:
@@ -769,11 +783,11 @@ def gated_recurrence_step(x, gate, state, form="leaky", new_state=None):
     if _wants_grad(x, gate, state):
         raise EngineError(f"{what}: no backward pass (use gated_recurrence, or torch.no_grad())")
     if new_state is None:
-        new_state = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+        new_state = torch.empty_like(x, dtype=torch.float32, memory_format=torch.contiguous_format)
     elif new_state.dtype != torch.float32 or new_state.shape != x.shape or not new_state.is_contiguous():
         raise EngineError(f"{what}: new_state must be contiguous float32 of x's shape {tuple(x.shape)}")
     x, gate, state = _contig(x), _contig(gate), _contig(state)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x)
     _call(x, "spk_recurrence_step", ptr(x), ptr(gate), dt, form, x.numel(), ptr(state), ptr(out), ptr(new_state))
     return out, new_state
 
@@ -786,10 +800,9 @@ def _group_norm_forward(x, groups, weight, bias, eps, act, thr, keep):
     """(y, mean, rstd) through spk_group_norm_act; mean and rstd [S, G] when `keep`."""
     lib = _lib.load()
     S, C = x.shape[0], x.shape[-1]
-    P = x[0].numel() // C if S else 0
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(S, groups, dtype=torch.float32, device=x.device) if keep else None
-    rstd = torch.empty_like(mean) if keep else None
+    P = x.numel() // (S * C) if S else 0
+    y = torch.empty_like(x)
+    mean, rstd = x.new_empty(2, S, groups, dtype=torch.float32) if keep else (None, None)
     ws = _scratch(x, lib.spk_group_norm_workspace_bytes(S, P, C, groups))
     _call(x, "spk_group_norm_act", ptr(x), _DTYPES[x.dtype], S, P, C, groups, ptr(weight), ptr(bias), eps, act, thr,
           ptr(y), ptr(mean), ptr(rstd), ptr(ws), 0 if ws is None else ws.numel())
@@ -804,17 +817,16 @@ class _GroupNormAct(torch.autograd.Function):
         ctx.groups, ctx.act, ctx.thr = groups, act, thr
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, gy):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         lib = _lib.load()
         gy = _contig(gy)
         S, C = x.shape[0], x.shape[-1]
-        P = x[0].numel() // C if S else 0
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dweight = torch.empty(C, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[1] else None
-        dbias = torch.empty(C, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
+        P = x.numel() // (S * C) if S else 0
+        dx = torch.empty_like(x)
+        dweight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        dbias = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
         ws = _scratch(x, lib.spk_group_norm_workspace_bytes(S, P, C, ctx.groups))
         _call(x, "spk_group_norm_act_backward", ptr(x), ptr(gy), _DTYPES[x.dtype], S, P, C, ctx.groups, ptr(weight),
               ptr(bias), ptr(mean), ptr(rstd), ctx.act, ctx.thr, ptr(dx), ptr(dweight), ptr(dbias), ptr(ws),
@@ -835,10 +847,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", thr=
     A (T, B, N, d) tensor is normalised per time plane and sample as
     x.flatten(0, 1).  Differentiable in x, weight and bias."""
     what = "group_norm_act"
-    require_cuda(x, weight, bias, what=what)
+    _checked(what, x, weight, bias)
     require_f32(weight, bias, what=what)
-    _dtype(x, what)
-    _same_device(x, weight, bias, what=what)
     if act not in _NORM_ACTS:
         raise EngineError(f"{what}: act must be one of {sorted(_NORM_ACTS)}")
     if x.dim() < 2 or x.shape[-1] == 0:
@@ -859,7 +869,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", thr=
 
 # ------------------------------------------------------------- dropout
 def _dropout_call(x, residual, p, key):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     dev = key if isinstance(key, torch.Tensor) else None
     seed, offset = (0, 0) if dev is not None else key
     _call(x, "spk_dropout", ptr(x), ptr(residual), _DTYPES[x.dtype], x.numel(), p, seed, offset, ptr(dev), ptr(y))
@@ -874,8 +884,7 @@ class _Dropout(torch.autograd.Function):
         ctx.save_for_backward(key if ctx.key is None else None)
         return _dropout_call(x, residual, p, key)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, gy):
         key = ctx.saved_tensors[0] if ctx.key is None else ctx.key
         gx = _dropout_call(_contig(gy), None, ctx.p, key) if ctx.needs_input_grad[0] else None
@@ -892,9 +901,7 @@ def dropout(x, p, key, residual=None):
     from the forward to the backward pass).  Give every call of a step its own
     offset.  Differentiable in x and residual."""
     what = "dropout"
-    require_cuda(x, residual, what=what)
-    _dtype(x, what)
-    _same_device(x, residual, what=what)
+    _checked(what, x, residual)
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise EngineError(f"{what}: p must lie in [0, 1], got {p}")
@@ -902,8 +909,7 @@ def dropout(x, p, key, residual=None):
         raise EngineError(f"{what}: residual must have x's shape and dtype ({tuple(x.shape)}, {x.dtype}), "
                           f"got {tuple(residual.shape)}, {residual.dtype}")
     if isinstance(key, torch.Tensor):
-        require_cuda(key, what=what)
-        _same_device(x, key, what=what)
+        _checked(what, x, key)
         if key.dtype != torch.int64 or key.shape != (2,):
             raise EngineError(f"{what}: key must be int64 of shape (2,), got {tuple(key.shape)}, {key.dtype}")
         key = _contig(key)
