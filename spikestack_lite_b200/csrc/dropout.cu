@@ -16,28 +16,33 @@ namespace spk {
 
 struct DropoutArgs {
   const void* x;
-  const void* r;         // or null
+  const void* r;          // or null
   void* y;
   int64_t n;
   uint64_t seed, offset;  // used when key is null
   const int64_t* key;     // (seed, offset) on the device, or null
-  uint64_t threshold;     // kept where word >= threshold (2^32: none)
+  uint32_t threshold;     // kept where word >= threshold
   float scale;
 };
 
 struct Philox7 {
-  uint32_t k0, k1, o0, o1;
+  uint32_t k0[7], k1[7], o0, o1;  // the rounds' keys, the counter's upper half
 
-  __device__ __forceinline__ Philox7(uint64_t seed, uint64_t offset)
-      : k0((uint32_t)seed), k1((uint32_t)(seed >> 32)), o0((uint32_t)offset), o1((uint32_t)(offset >> 32)) {}
+  __device__ __forceinline__ Philox7(uint64_t seed, uint64_t offset) : o0((uint32_t)offset), o1((uint32_t)(offset >> 32)) {
+#pragma unroll
+    for (int r = 0; r < 7; ++r) {
+      k0[r] = (uint32_t)seed + (uint32_t)r * 0x9E3779B9u;
+      k1[r] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
+    }
+  }
 
   __device__ __forceinline__ uint4 operator()(uint64_t counter) const {
     uint32_t c0 = (uint32_t)counter, c1 = (uint32_t)(counter >> 32), c2 = o0, c3 = o1;
 #pragma unroll
     for (int r = 0; r < 7; ++r) {
       const uint64_t m0 = (uint64_t)c0 * 0xD2511F53u, m1 = (uint64_t)c2 * 0xCD9E8D57u;
-      const uint32_t n0 = (uint32_t)(m1 >> 32) ^ c1 ^ (k0 + (uint32_t)r * 0x9E3779B9u);
-      const uint32_t n2 = (uint32_t)(m0 >> 32) ^ c3 ^ (k1 + (uint32_t)r * 0xBB67AE85u);
+      const uint32_t n0 = (uint32_t)(m1 >> 32) ^ c1 ^ k0[r];
+      const uint32_t n2 = (uint32_t)(m0 >> 32) ^ c3 ^ k1[r];
       c1 = (uint32_t)m1;
       c3 = (uint32_t)m0;
       c0 = n0;
@@ -47,57 +52,84 @@ struct Philox7 {
   }
 };
 
-// A thread takes V = 4 or 8 consecutive elements (16 bytes) at a time: V / 4
-// counters.  ALIGNED: every tensor is 16-byte aligned and the accesses are
-// 16 bytes wide; otherwise they are single elements, of the same counters.
-template <typename E, bool ALIGNED>
-__global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a) {
+constexpr int kDropThreads = 256;
+
+template <typename E, bool RES, int V>
+__device__ __forceinline__ Pack<E, V> dropout_pack(const Pack<E, V>& x, const Pack<E, V>& r, const Philox7& rng,
+                                                   int64_t i, uint32_t threshold, float scale) {
+  float y[V];
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    const uint4 w = rng((uint64_t)(i * (V / 4) + q));
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // a dropped element contributes 0 whatever it holds (no inf * 0)
+      const float v = ws[j] >= threshold ? elem_to_f32(x.e[4 * q + j]) : 0.0f;
+      y[4 * q + j] = RES ? fmaf(v, scale, elem_to_f32(r.e[4 * q + j])) : v * scale;
+    }
+  }
+  return pack_f32<E, V>(y);
+}
+
+// A thread takes U packs of V = 4 or 8 consecutive elements (16 bytes, V / 4
+// counters) at a time.  ALIGNED: every tensor is 16-byte aligned and the
+// accesses are 16 bytes wide; otherwise they are single elements, of the same
+// counters.  The last, partial pack goes by elements too.
+template <typename E, bool RES, bool ALIGNED, int U>
+__global__ void __launch_bounds__(kDropThreads) dropout_kernel(DropoutArgs a) {
   constexpr int V = 16 / (int)sizeof(E);
   const uint64_t seed = a.key != nullptr ? (uint64_t)a.key[0] : a.seed;
   const uint64_t offset = a.key != nullptr ? (uint64_t)a.key[1] : a.offset;
   const Philox7 rng(seed, offset);
-  const E* X = static_cast<const E*>(a.x);
-  const E* R = static_cast<const E*>(a.r);
-  E* Y = static_cast<E*>(a.y);
-  const bool none = a.threshold > 0xffffffffull;
-  const uint32_t thr = (uint32_t)a.threshold;
-  const int64_t vecs = ceil_div(a.n, V), step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < vecs; i += step) {
-    const int64_t at = i * V;
-    const bool whole = at + V <= a.n;
-    Pack<E, V> x, r, y;
-    if (ALIGNED && whole) {
-      x = load_pack<E, V>(X + at);
-      if (R != nullptr) r = load_pack<E, V>(R + at);
-    } else {
+  const E* const X = static_cast<const E*>(a.x);
+  const E* const R = static_cast<const E*>(a.r);
+  E* const Y = static_cast<E*>(a.y);
+  const int64_t whole = ALIGNED ? a.n / V : 0;
+  const int64_t step = (int64_t)gridDim.x * kDropThreads * U;
+  for (int64_t i0 = (int64_t)blockIdx.x * kDropThreads * U + threadIdx.x; i0 < whole; i0 += step) {
+    Pack<E, V> x[U], r[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (at + j < a.n) {
-          x.e[j] = X[at + j];
-          if (R != nullptr) r.e[j] = R[at + j];
-        }
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * kDropThreads;
+      if (i < whole) {
+        x[u] = load_pack<E, V>(X + i * V);
+        if (RES) r[u] = load_pack<E, V>(R + i * V);
       }
     }
 #pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const uint4 w = rng((uint64_t)(i * (V / 4) + q));
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool keep = ws[j] >= thr && !none;
-        // a dropped element contributes 0 whatever it holds (no inf * 0)
-        const float v = keep ? elem_to_f32(x.e[4 * q + j]) : 0.0f;
-        y.e[4 * q + j] = elem_from_f32<E>(R != nullptr ? fmaf(v, a.scale, elem_to_f32(r.e[4 * q + j])) : v * a.scale);
-      }
-    }
-    if (ALIGNED && whole) {
-      store_pack<E, V>(Y + at, y);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (at + j < a.n) Y[at + j] = y.e[j];
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * kDropThreads;
+      if (i < whole) store_pack<E, V>(Y + i * V, dropout_pack<E, RES, V>(x[u], r[u], rng, i, a.threshold, a.scale));
     }
   }
+  const int64_t vecs = ceil_div(a.n, V);
+  for (int64_t i = whole + (int64_t)blockIdx.x * kDropThreads + threadIdx.x; i < vecs;
+       i += (int64_t)gridDim.x * kDropThreads) {
+    Pack<E, V> x, r;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const bool in = i * V + j < a.n;
+      x.e[j] = in ? X[i * V + j] : elem_from_f32<E>(0.0f);
+      r.e[j] = RES && in ? R[i * V + j] : elem_from_f32<E>(0.0f);
+    }
+    const Pack<E, V> y = dropout_pack<E, RES, V>(x, r, rng, i, a.threshold, a.scale);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (i * V + j < a.n) Y[i * V + j] = y.e[j];
+  }
+}
+
+template <typename E, bool RES>
+static void dropout_launch(const DropoutArgs& a, bool aligned, cudaStream_t st) {
+  const int64_t vecs = ceil_div(a.n, (int64_t)(16 / sizeof(E))), most = (int64_t)sm_count() * 8;
+  const unsigned blocks = (unsigned)min64(ceil_div(vecs, kDropThreads), most);
+  if (!aligned)
+    dropout_kernel<E, RES, false, 1><<<blocks, kDropThreads, 0, st>>>(a);
+  else if (vecs <= most * kDropThreads)
+    dropout_kernel<E, RES, true, 1><<<blocks, kDropThreads, 0, st>>>(a);
+  else
+    dropout_kernel<E, RES, true, 2><<<blocks, kDropThreads, 0, st>>>(a);
 }
 
 }  // namespace spk
@@ -112,6 +144,15 @@ extern "C" int spk_dropout(const void* X, const void* R, int dtype, int64_t n, d
   SPK_REQUIRE(X != nullptr && Y != nullptr, "X and Y must be non-null");
   SPK_REQUIRE(spk::aligned_to(X, eb) && spk::aligned_to(R, eb) && spk::aligned_to(Y, eb) && spk::aligned_to(key, 8),
               "tensors must be aligned to their elements");
+  cudaStream_t st = (cudaStream_t)stream;
+  const uint64_t threshold = (uint64_t)(p * 4294967296.0 + 0.5);
+  if (threshold > 0xffffffffull) {  // nothing is kept
+    if (R == nullptr)
+      SPK_CUDA_TRY(cudaMemsetAsync(Y, 0, (size_t)n * eb, st));
+    else if (Y != R)
+      SPK_CUDA_TRY(cudaMemcpyAsync(Y, R, (size_t)n * eb, cudaMemcpyDeviceToDevice, st));
+    return SPK_OK;
+  }
   spk::DropoutArgs a{};
   a.x = X;
   a.r = R;
@@ -120,18 +161,15 @@ extern "C" int spk_dropout(const void* X, const void* R, int dtype, int64_t n, d
   a.seed = seed;
   a.offset = offset;
   a.key = key;
-  a.threshold = (uint64_t)(p * 4294967296.0 + 0.5);
-  a.scale = a.threshold <= 0xffffffffull ? (float)(1.0 / (1.0 - p)) : 0.0f;  // nothing kept: 0, not 0 * inf
+  a.threshold = (uint32_t)threshold;
+  a.scale = (float)(1.0 / (1.0 - p));
   const bool aligned = spk::aligned_to(X, 16) && spk::aligned_to(R, 16) && spk::aligned_to(Y, 16);
-  const int64_t vecs = spk::ceil_div(n, (int64_t)(16 / eb));
-  const int64_t blocks = spk::min64(spk::ceil_div(vecs, 256), (int64_t)spk::sm_count() * 8);
-  cudaStream_t st = (cudaStream_t)stream;
   spk::with_elem(dtype, [&](auto e) {
     using E = decltype(e);
-    if (aligned)
-      spk::dropout_kernel<E, true><<<(unsigned)blocks, 256, 0, st>>>(a);
+    if (R != nullptr)
+      spk::dropout_launch<E, true>(a, aligned, st);
     else
-      spk::dropout_kernel<E, false><<<(unsigned)blocks, 256, 0, st>>>(a);
+      spk::dropout_launch<E, false>(a, aligned, st);
   });
   SPK_LAUNCH_CHECK();
   spk::count_launch(1);

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "spk_common.cuh"
 
@@ -44,6 +45,28 @@ __device__ __forceinline__ Pack<E, V> load_pack(const E* p) {
 template <typename E, int V>
 __device__ __forceinline__ void store_pack(E* p, const Pack<E, V>& v) {
   *reinterpret_cast<Pack<E, V>*>(p) = v;
+}
+
+// V fp32 values rounded to E; 16-bit ones in pairs, one conversion each.
+template <typename E, int V>
+__device__ __forceinline__ Pack<E, V> pack_f32(const float (&v)[V]) {
+  Pack<E, V> p;
+#pragma unroll
+  for (int i = 0; i + 1 < V; i += 2) {
+    if constexpr (sizeof(E) == 4) {
+      p.e[i] = v[i];
+      p.e[i + 1] = v[i + 1];
+    } else {
+      uint32_t w;
+      if constexpr (std::is_same_v<E, __half>)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(v[i + 1]), "f"(v[i]));
+      else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(v[i + 1]), "f"(v[i]));
+      reinterpret_cast<uint32_t*>(&p)[i / 2] = w;
+    }
+  }
+  if (V % 2) p.e[V - 1] = elem_from_f32<E>(v[V - 1]);
+  return p;
 }
 
 // The hardware's exponential of two and reciprocal (relative errors of 2^-22

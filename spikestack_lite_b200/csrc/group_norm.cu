@@ -131,12 +131,11 @@ __device__ __forceinline__ void gn_affine(const GnArgs& a, int64_t s, int c0, Gn
 
 template <typename E, int ACT, int V, int M>
 __device__ __forceinline__ Pack<E, V> gn_forward(const Pack<E, V>& x, const GnAffine<V, M>& f, float thr) {
-  Pack<E, V> y;
+  float y[V];
 #pragma unroll
   for (int j = 0; j < V; ++j)
-    y.e[j] = elem_from_f32<E>(
-        gn_act<E, ACT>(fmaf(elem_to_f32(x.e[j]) - f.mean[M > 1 ? j : 0], f.a[j], f.b[j]), thr));
-  return y;
+    y[j] = gn_act<E, ACT>(fmaf(elem_to_f32(x.e[j]) - f.mean[M > 1 ? j : 0], f.a[j], f.b[j]), thr);
+  return pack_f32<E, V>(y);
 }
 
 // dz and d of one element.
@@ -156,15 +155,15 @@ __device__ __forceinline__ float2 gn_pull(float2 m, float rstd) {
 template <typename E, int ACT, int V, int M>
 __device__ __forceinline__ Pack<E, V> gn_backward(const Pack<E, V>& x, const Pack<E, V>& gy,
                                                   const GnAffine<V, M>& f, const float2 (&k)[M], float thr) {
-  Pack<E, V> o;
+  float o[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float d;
     const float dz = gn_dz<E, ACT, V, M>(x, gy, f, j, thr, &d);
     const float2 kj = k[M > 1 ? j : 0];
-    o.e[j] = elem_from_f32<E>(fmaf(dz, f.a[j], fmaf(d, kj.y, kj.x)));
+    o[j] = fmaf(dz, f.a[j], fmaf(d, kj.y, kj.x));
   }
-  return o;
+  return pack_f32<E, V>(o);
 }
 
 // ---- resident form: a block holds a sample's k groups (all positions) in
@@ -369,14 +368,13 @@ __global__ void __launch_bounds__(kGnThreads, N > 2 ? 2 : 3) gn_resident_backwar
   for (int i = 0; i < N; ++i)
     if (i < rows) {
       if (kKeep) {
-        Pack<E, V> o;
+        float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float2 kj = k[M > 1 ? j : 0];
-          o.e[j] = elem_from_f32<E>(
-              fmaf(keep_dz[kKeep ? i : 0][j], f.a[j], fmaf(keep_d[kKeep ? i : 0][j], kj.y, kj.x)));
+          o[j] = fmaf(keep_dz[kKeep ? i : 0][j], f.a[j], fmaf(keep_d[kKeep ? i : 0][j], kj.y, kj.x));
         }
-        store_pack<E, V>(dx + i * step, o);
+        store_pack<E, V>(dx + i * step, pack_f32<E, V>(o));
       } else {
         store_pack<E, V>(dx + i * step, gn_backward<E, ACT, V, M>(x[i], gy[i], f, k, a.thr));
       }

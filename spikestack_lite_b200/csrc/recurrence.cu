@@ -239,12 +239,7 @@ __device__ __forceinline__ Cols<V> rec_load(const E* p, int lane, int n, float o
 template <int V, bool ALIGNED, typename E>
 __device__ __forceinline__ void rec_store(E* p, int lane, int n, const Cols<V>& q) {
   if (ALIGNED) {
-    if (V * lane < n) {
-      Pack<E, V> e;
-#pragma unroll
-      for (int i = 0; i < V; ++i) e.e[i] = elem_from_f32<E>(q.v[i]);
-      store_pack<E, V>(p + V * lane, e);
-    }
+    if (V * lane < n) store_pack<E, V>(p + V * lane, pack_f32<E, V>(q.v));
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
