@@ -82,6 +82,11 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 
+// Programmatic dependent launch: the next kernel of the stream may start when
+// every block has said so; what the previous one wrote is there after the wait.
+__device__ __forceinline__ void grid_dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 inline size_t elem_bytes(int dtype) { return dtype == SPK_F32 ? 4 : (dtype == SPK_BF16 || dtype == SPK_F16) ? 2 : 0; }
 
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

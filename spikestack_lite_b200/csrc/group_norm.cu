@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(kGnThreads, N > 2 ? 2 : 3) gn_resident_backwar
   constexpr int V = 16 / (int)sizeof(E), M = WHOLE ? 1 : V;
   extern __shared__ __align__(16) unsigned char gn_smem[];
   float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][width] sums of dz and dz xhat
+  grid_dependents_may_start();
   const int64_t s = blockIdx.x / a.tiles;
   const int g0 = (int)(blockIdx.x - s * a.tiles) * a.k, ng = min(a.k, a.G - g0), width = ng * a.cg;
   GnSpot q = gn_spot(V, a.tpr, a.rpp);
@@ -410,6 +411,7 @@ __global__ void __launch_bounds__(kGnThreads, 4) gn_stats_kernel(GnArgs a) {
   float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][tpr V]
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
   const GnTile t = gn_tile<V>(a, blockIdx.x, q);
+  grid_dependents_may_start();
   float mean[V], m2[V], n = 0.0f;
 #pragma unroll
   for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.0f;
@@ -475,27 +477,41 @@ __device__ __forceinline__ float gn_block_sum(float v, float* sm) {
   return r;
 }
 
+// The parts of one group, every kGnThreads-th from this thread's on: f(tile, channel).
+template <typename F>
+__device__ __forceinline__ void gn_each_part(const GnArgs& a, F&& f) {
+  const int down = kGnThreads / a.cg, right = kGnThreads - down * a.cg;
+  int t = (int)threadIdx.x / a.cg, c = (int)threadIdx.x - t * a.cg;
+#pragma unroll 4
+  for (; t < a.tiles; t += down) {
+    f(t, c);
+    c += right;
+    if (c >= a.cg) {
+      c -= a.cg;
+      ++t;
+    }
+  }
+}
+
 // One block per (sample, group): joins the tiles' moments.
 __global__ void __launch_bounds__(kGnThreads) gn_stats_finish_kernel(GnArgs a) {
   __shared__ float sm[kGnThreads / 32];
+  grid_dependents_may_start();
+  grid_wait_for_previous();
   const int64_t u = blockIdx.x, s = u / a.G, g = u - s * a.G;
-  const int64_t parts = (int64_t)a.tiles * a.cg;
   const float2* part = reinterpret_cast<const float2*>(a.part) + s * a.tiles * a.C + g * a.cg;
-  const float total = (float)a.P * (float)a.cg;
+  const float total = (float)a.P * (float)a.cg, rows = (float)a.rows;
+  const float tail = (float)(int)(a.P - (int64_t)(a.tiles - 1) * a.rows);  // rows of the last tile
   float sum = 0.0f, m2 = 0.0f;
-  for (int64_t i = threadIdx.x; i < parts; i += kGnThreads) {
-    const int t = (int)(i / a.cg);
-    const float n = (float)(int)min64(a.rows, a.P - (int64_t)t * a.rows);
-    sum = fmaf(n, part[(int64_t)t * a.C + (i - (int64_t)t * a.cg)].x, sum);
-  }
+  gn_each_part(a, [&](int t, int c) {
+    sum = fmaf(t + 1 < a.tiles ? rows : tail, part[(int64_t)t * a.C + c].x, sum);
+  });
   const float mean = gn_block_sum<kGnThreads>(sum, sm) / total;
-  for (int64_t i = threadIdx.x; i < parts; i += kGnThreads) {
-    const int t = (int)(i / a.cg);
-    const float n = (float)(int)min64(a.rows, a.P - (int64_t)t * a.rows);
-    const float2 v = part[(int64_t)t * a.C + (i - (int64_t)t * a.cg)];
+  gn_each_part(a, [&](int t, int c) {
+    const float2 v = part[(int64_t)t * a.C + c];
     const float d = v.x - mean;
-    m2 += fmaf(n * d, d, v.y);
-  }
+    m2 += fmaf((t + 1 < a.tiles ? rows : tail) * d, d, v.y);
+  });
   const float var = gn_block_sum<kGnThreads>(m2, sm) / total;
   if (threadIdx.x == 0) {
     a.mean[u] = mean;
@@ -507,6 +523,8 @@ template <typename E, int ACT, int V, int M>
 __global__ void __launch_bounds__(kGnThreads, 4) gn_apply_kernel(GnArgs a) {
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
   const GnTile t = gn_tile<V>(a, gridDim.x - 1 - (int64_t)blockIdx.x, q);
+  grid_dependents_may_start();
+  grid_wait_for_previous();
   if (!t.live) return;
   GnAffine<V, M> f;
   gn_affine<V, M>(a, t.s, t.c0, &f);
@@ -532,6 +550,7 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_grad_sums_kernel(GnArgs a) {
   float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][tpr V]
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
   const GnTile t = gn_tile<V>(a, blockIdx.x, q);
+  grid_dependents_may_start();
   if (t.live) {
     GnAffine<V, M> f;
     gn_affine<V, M>(a, t.s, t.c0, &f);
@@ -578,17 +597,18 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_grad_sums_kernel(GnArgs a) {
 // One block per (sample, group): mean(dn) and mean(dn xhat).
 __global__ void __launch_bounds__(kGnThreads) gn_grad_finish_kernel(GnArgs a) {
   __shared__ float sm[kGnThreads / 32];
+  grid_dependents_may_start();
+  grid_wait_for_previous();
   const int64_t u = blockIdx.x, s = u / a.G, g = u - s * a.G;
-  const int64_t parts = (int64_t)a.tiles * a.cg;
   const float2* part = reinterpret_cast<const float2*>(a.part) + s * a.tiles * a.C + g * a.cg;
+  const float* weight = a.weight != nullptr ? a.weight + g * a.cg : nullptr;
   float s1 = 0.0f, s2 = 0.0f;
-  for (int64_t i = threadIdx.x; i < parts; i += kGnThreads) {
-    const int t = (int)(i / a.cg), c = (int)(i - (int64_t)t * a.cg);
-    const float w = a.weight != nullptr ? a.weight[g * a.cg + c] : 1.0f;
+  gn_each_part(a, [&](int t, int c) {
+    const float w = weight != nullptr ? weight[c] : 1.0f;
     const float2 v = part[(int64_t)t * a.C + c];
     s1 = fmaf(w, v.x, s1);
     s2 = fmaf(w, v.y, s2);
-  }
+  });
   s1 = gn_block_sum<kGnThreads>(s1, sm);
   s2 = gn_block_sum<kGnThreads>(s2, sm);
   if (threadIdx.x == 0) {
@@ -602,6 +622,8 @@ template <typename E, int ACT, int V, int M>
 __global__ void __launch_bounds__(kGnThreads, 3) gn_grad_apply_kernel(GnArgs a) {
   const GnSpot q = gn_spot(V, a.tpr, a.rpp);
   const GnTile t = gn_tile<V>(a, gridDim.x - 1 - (int64_t)blockIdx.x, q);
+  grid_dependents_may_start();
+  grid_wait_for_previous();
   if (!t.live) return;
   GnAffine<V, M> f;
   gn_affine<V, M>(a, t.s, t.c0, &f);
@@ -633,6 +655,7 @@ __global__ void __launch_bounds__(kGnThreads, 3) gn_grad_apply_kernel(GnArgs a) 
 // order (the same bits on every run).  32 channels per block, 32 threads each.
 __global__ void __launch_bounds__(1024) gn_param_grad_kernel(GnArgs a) {
   __shared__ float2 sm[32][33];
+  grid_wait_for_previous();
   const int c = blockIdx.x * 32 + threadIdx.x;
   float2 acc = make_float2(0.0f, 0.0f);
   if (c < a.C) {
@@ -698,16 +721,18 @@ static size_t gn_resident_smem(const GnArgs& a, int V, bool whole, bool backward
 }
 
 // Tiled form: blocks of up to 256 threads whose rows waste the fewest of them,
-// tiles of at least 32 positions (the partial sums stay well below the tensor)
-// and enough of them for the GPU.
-static void gn_tiled_rows(int64_t S, int64_t P, int C, int* rows, int* tiles) {
-  const int64_t want = ceil_div(148 * 4, max64(S, 1));
-  const int64_t r = max64(32, max64(ceil_div(P, want), ceil_div(P, 65535)));
+// and `per_sm` of them on an SM at once: one wave of tiles where the samples
+// divide it, else several of smaller ones; at least 32 positions each (the
+// partial sums stay well below the tensor).
+static void gn_tiled_rows(int64_t S, int64_t P, int per_sm, int* rows, int* tiles) {
+  const int64_t slots = 148 * (int64_t)per_sm;
+  const int64_t t = S * 8 <= slots ? slots / max64(S, 1) : ceil_div(4 * slots, S);
+  const int64_t r = max64(32, max64(ceil_div(P, t), ceil_div(P, 65535)));
   *rows = (int)min64(r, max64(P, 1));
   *tiles = (int)ceil_div(max64(P, 1), *rows);
 }
 
-static void gn_tiled_plan(GnArgs* a, int V) {
+static void gn_tiled_plan(GnArgs* a, int V, int per_sm) {
   const int per_row = (int)ceil_div(a->C, V);
   a->tpr = per_row > kGnThreads ? kGnThreads : per_row;
   a->rpp = 1;
@@ -716,20 +741,21 @@ static void gn_tiled_plan(GnArgs* a, int V) {
   for (int rpp = 1; rpp * a->tpr <= kGnThreads && rpp <= 64; ++rpp) {
     const int threads = 32 * (int)ceil_div(rpp * a->tpr, 32);
     const double used = (double)(rpp * a->tpr) / threads * (threads >= 192 ? 1.0 : threads / 192.0);
-    if (used > best + 1e-9) {
+    if (used > best - 1e-9) {  // of equals the larger
       best = used;
       a->rpp = rpp;
       a->threads = threads;
     }
   }
-  gn_tiled_rows(a->S, a->P, a->C, &a->rows, &a->tiles);
+  gn_tiled_rows(a->S, a->P, per_sm, &a->rows, &a->tiles);
   a->parts = a->S * a->tiles;
 }
 
 static size_t gn_part_bytes(int64_t S, int64_t P, int C) {
-  int rows, tiles;
-  gn_tiled_rows(S, P, C, &rows, &tiles);
-  return align_up((size_t)S * tiles * C * 2 * sizeof(float), 256);
+  int rows, tiles = 0, fewer;
+  gn_tiled_rows(S, P, 4, &rows, &tiles);
+  gn_tiled_rows(S, P, 3, &rows, &fewer);
+  return align_up((size_t)S * (tiles > fewer ? tiles : fewer) * C * 2 * sizeof(float), 256);
 }
 
 static int gn_check(int dtype, int64_t S, int64_t P, int C, int G, int act, size_t* eb) {
@@ -743,7 +769,7 @@ static int gn_check(int dtype, int64_t S, int64_t P, int C, int G, int act, size
   SPK_REQUIRE(C <= (1 << 20) && P < (1ll << 31) && S * G < (1ll << 31) && (P == 0 || S < (1ll << 42) / ((int64_t)C * P)),
               "shape too large (S=%lld, P=%lld, C=%d)", (long long)S, (long long)P, C);
   int rows, tiles;
-  gn_tiled_rows(S, P, C, &rows, &tiles);
+  gn_tiled_rows(S, P, 4, &rows, &tiles);
   SPK_REQUIRE(S * tiles < (1ll << 31), "too many positions (S=%lld, P=%lld)", (long long)S, (long long)P);
   return SPK_OK;
 }
@@ -838,7 +864,13 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
     spk::count_launch(1);
     return SPK_OK;
   }
-  spk::gn_tiled_plan(&a, V);
+  spk::gn_tiled_plan(&a, V, 4);
+  // a kernel that starts while the one before it drains
+  cudaError_t rc = cudaSuccess;
+  auto launch = [&](auto kernel, dim3 grid, dim3 block) {
+    const cudaError_t e = spk::launch_dependent(kernel, grid, block, 0, st, a);
+    if (rc == cudaSuccess) rc = e;
+  };
   const dim3 grid((unsigned)a.parts, (unsigned)spk::ceil_div(C, a.tpr * V)), block((unsigned)a.threads);
   const size_t smem = (size_t)a.rpp * a.tpr * V * sizeof(float2);
   spk::with_elem(dtype, [&](auto e) {
@@ -846,12 +878,13 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
     spk::with_gn_vector<E>(V, a.cg, [&](auto vc, auto mc) {
       constexpr int VV = decltype(vc)::value, MM = decltype(mc)::value;
       spk::gn_stats_kernel<E, VV><<<grid, block, smem, st>>>(a);
-      spk::gn_stats_finish_kernel<<<(unsigned)(S * G), spk::kGnThreads, 0, st>>>(a);
+      launch(spk::gn_stats_finish_kernel, dim3((unsigned)(S * G)), dim3(spk::kGnThreads));
       spk::with_gn_act(act, [&](auto ac) {
-        spk::gn_apply_kernel<E, decltype(ac)::value, VV, MM><<<grid, block, 0, st>>>(a);
+        launch(spk::gn_apply_kernel<E, decltype(ac)::value, VV, MM>, grid, block);
       });
     });
   });
+  SPK_CUDA_TRY(rc);
   SPK_LAUNCH_CHECK();
   spk::count_launch(3);
   return SPK_OK;
@@ -901,6 +934,12 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
   a.thr = thr;
   const int V = spk::gn_vector(eb, C, X, GY, DX);
   const bool params = dweight != nullptr || dbias != nullptr;
+  // a kernel that starts while the one before it drains
+  cudaError_t rc = cudaSuccess;
+  auto launch = [&](auto kernel, dim3 grid, dim3 block) {
+    const cudaError_t e = spk::launch_dependent(kernel, grid, block, 0, st, a);
+    if (rc == cudaSuccess) rc = e;
+  };
   if (spk::gn_resident_plan(&a, eb, V, 2) || spk::gn_resident_plan(&a, eb, V, 8)) {
     const size_t smem = spk::gn_resident_smem(a, V, false, true);
     const bool whole = a.cg % V == 0;
@@ -923,7 +962,7 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
     });
     spk::count_launch(1);
   } else {
-    spk::gn_tiled_plan(&a, V);
+    spk::gn_tiled_plan(&a, V, 3);
     const dim3 grid((unsigned)a.parts, (unsigned)spk::ceil_div(C, a.tpr * V)), block((unsigned)a.threads);
     const size_t smem = (size_t)a.rpp * a.tpr * V * sizeof(float2);
     spk::with_elem(dtype, [&](auto e) {
@@ -933,17 +972,18 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
         spk::with_gn_act(act, [&](auto ac) {
           constexpr int ACT = decltype(ac)::value;
           spk::gn_grad_sums_kernel<E, ACT, VV, MM><<<grid, block, smem, st>>>(a);
-          spk::gn_grad_finish_kernel<<<(unsigned)(S * G), spk::kGnThreads, 0, st>>>(a);
-          spk::gn_grad_apply_kernel<E, ACT, VV, MM><<<grid, block, 0, st>>>(a);
+          launch(spk::gn_grad_finish_kernel, dim3((unsigned)(S * G)), dim3(spk::kGnThreads));
+          launch(spk::gn_grad_apply_kernel<E, ACT, VV, MM>, grid, block);
         });
       });
     });
     spk::count_launch(3);
   }
   if (params) {
-    spk::gn_param_grad_kernel<<<(unsigned)spk::ceil_div(C, 32), dim3(32, 32), 0, st>>>(a);
+    launch(spk::gn_param_grad_kernel, dim3((unsigned)spk::ceil_div(C, 32)), dim3(32, 32));
     spk::count_launch(1);
   }
+  SPK_CUDA_TRY(rc);
   SPK_LAUNCH_CHECK();
   return SPK_OK;
 }
