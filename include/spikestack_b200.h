@@ -349,10 +349,12 @@ int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_t x_stride_
                             const float* state, const int32_t* lengths, const float* carry, const float* glast,
                             void* dx, void* dgate, int64_t d_stride_b, int64_t d_stride_t, float* dstate,
                             spk_stream_t stream);
-/* One step over n cells (all contiguous): out [n] dtype, new_state [n] fp32
- * (may be state itself). */
-int spk_recurrence_step(const void* x, const void* gate, int dtype, int form, int64_t n, const float* state,
-                        void* out, float* new_state, spk_stream_t stream);
+/* One step over `rows` rows of D cells: x and gate with a row stride (in
+ * elements; their cells contiguous), state, out (dtype) and new_state (fp32,
+ * may be state itself) contiguous. */
+int spk_recurrence_step(const void* x, int64_t x_stride, const void* gate, int64_t g_stride, int dtype, int form,
+                        int64_t rows, int64_t D, const float* state, void* out, float* new_state,
+                        spk_stream_t stream);
 
 /* ------------------------------------------------------- group norm + activation
  * Group norm on channels-last X [S, P, C] with act SPK_ACT_NONE,

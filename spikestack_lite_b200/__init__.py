@@ -4,7 +4,8 @@ Hand-written CUDA kernels behind a C ABI (include/spikestack_b200.h,
 libspk_b200.so) with a thin PyTorch host that mirrors the reference's own
 API: ``sparse`` (spike-linear ops, SparseLinear), ``attention``
 (AstrocyteHebbianAttention, SpikingFFN, AstrocyteHebbianBlock), ``gsmc``
-(FusedGSMC) and ``transformer`` (SpikingTransformer host composition);
+(FusedGSMC), ``recurrence`` (GatedRecurrence, Dropout: training and streaming)
+and ``transformer`` (SpikingTransformer host composition);
 ``engine`` holds drop-in engine objects with the reference's pybind names and
 ``engine.install(spikestack_lite)`` swaps them into an imported reference.
 """

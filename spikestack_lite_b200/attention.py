@@ -19,6 +19,7 @@ from . import ops
 from .ops import engine_linear
 from ._lib import EngineError
 from .engine import attention_engine
+from .recurrence import Dropout
 from .sparse import SparseLinear
 
 _attn_cuda_engine = attention_engine
@@ -214,15 +215,19 @@ class SpikingFFN(nn.Module):
 
 
 class AstrocyteHebbianBlock(nn.Module):
-    """Pre-norm block: x + attn(LN(x)), then x + ffn(LN(x)) (attention.py:162-177)."""
+    """Pre-norm block: x + attn(LN(x)), then x + ffn(LN(x)) (attention.py:162-177).
+    ``dropout`` > 0 (no reference counterpart): in training mode both branches
+    pass the counter-based dropout, added to the residual in one pass."""
 
     def __init__(self, d_model=128, num_heads=4, expansion=4, v_levels=1, use_spikeskip=False,
-                 spike_threshold=0.0):
+                 spike_threshold=0.0, dropout=0.0):
         super().__init__()
         self.norm1 = nn.LayerNorm(d_model)
         self.attn = AstrocyteHebbianAttention(d_model, num_heads, v_levels)
         self.norm2 = nn.LayerNorm(d_model)
         self.ffn = SpikingFFN(d_model, expansion, use_spikeskip=use_spikeskip, spike_threshold=spike_threshold)
+        self.drop_attn = Dropout(dropout) if dropout > 0.0 else None
+        self.drop_ffn = Dropout(dropout) if dropout > 0.0 else None
 
     def forward(self, x):
         return self.forward_fused(x)[0]
@@ -234,6 +239,11 @@ class AstrocyteHebbianBlock(nn.Module):
         block's norm1), whose result the caller hands back as `x_norm`.
         ``record`` (a dict, optional) receives the stages: q, k, v, attn, the
         mid-block residual "x_mid" and the fc1 spikes "act"."""
+        if self.drop_attn is not None and self.training:
+            x = self.drop_attn(self.attn(self.norm1(x), record), residual=x)
+            if record is not None:
+                record["x_mid"] = x
+            return self.drop_ffn(self.ffn(self.norm2(x), record), residual=x), None
         if not _engine_norm_ok(self.norm1, x):  # the reference's composition (autograd, CPU)
             x = x + self.attn(self.norm1(x), record)
             if record is not None:

@@ -791,15 +791,18 @@ __global__ void __launch_bounds__(kRecThreads, 2) recurrence_long_backward_kerne
   if (K > 1) cluster_sync_all();  // maps may still be on their way here
 }
 
-// One step of the recurrence over n cells: out (element type) and the new
-// state (fp32; may be the old state's own buffer).
+// One step of the recurrence over rows of D cells: out (element type) and the
+// new state (fp32; may be the old state's own buffer).
 template <typename E, typename Form>
-__global__ void __launch_bounds__(256) recurrence_step_kernel(const E* __restrict__ x, const E* __restrict__ gate,
-                                                              const float* state, int64_t n, E* __restrict__ out,
-                                                              float* new_state) {
+__global__ void __launch_bounds__(256) recurrence_step_kernel(const E* __restrict__ x, int64_t x_stride,
+                                                              const E* __restrict__ gate, int64_t g_stride,
+                                                              const float* state, int64_t n, int D,
+                                                              E* __restrict__ out, float* new_state) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n) return;
-  const float h = Form::step(state[i], Form::coeff(elem_to_f32(gate[i])), elem_to_f32(x[i]));
+  const int64_t r = i / D, d = i - r * D;
+  const float h =
+      Form::step(state[i], Form::coeff(elem_to_f32(gate[r * g_stride + d])), elem_to_f32(x[r * x_stride + d]));
   out[i] = elem_from_f32<E>(h);
   new_state[i] = h;
 }
@@ -1063,22 +1066,24 @@ extern "C" int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_
   return spk::rec_run(true, dtype, form, aligned, a, p, st);
 }
 
-extern "C" int spk_recurrence_step(const void* x, const void* gate, int dtype, int form, int64_t n,
-                                   const float* state, void* out, float* new_state, spk_stream_t stream) {
+extern "C" int spk_recurrence_step(const void* x, int64_t x_stride, const void* gate, int64_t g_stride, int dtype,
+                                   int form, int64_t rows, int64_t D, const float* state, void* out, float* new_state,
+                                   spk_stream_t stream) {
   size_t eb = 0;
-  if (int rc = spk::rec_check(dtype, form, n, 1, 1, &eb)) return rc;
-  if (n == 0) return SPK_OK;
+  if (int rc = spk::rec_check(dtype, form, rows, 1, D, &eb)) return rc;
+  if (rows == 0 || D == 0) return SPK_OK;
   SPK_REQUIRE(x != nullptr && gate != nullptr && state != nullptr && out != nullptr && new_state != nullptr,
               "x, gate, state, out and new_state must be non-null");
   SPK_REQUIRE(spk::aligned_to(x, eb) && spk::aligned_to(gate, eb) && spk::aligned_to(out, eb) &&
                   spk::aligned_to(state, 4) && spk::aligned_to(new_state, 4),
               "tensors must be aligned to their elements");
-  const unsigned blocks = (unsigned)spk::ceil_div(n, 256);
+  const unsigned blocks = (unsigned)spk::ceil_div(rows * D, 256);
   spk::with_elem(dtype, [&](auto e) {
     using E = decltype(e);
     spk::with_form<E>(form, [&](auto f) {
       spk::recurrence_step_kernel<E, decltype(f)><<<blocks, 256, 0, (cudaStream_t)stream>>>(
-          static_cast<const E*>(x), static_cast<const E*>(gate), state, n, static_cast<E*>(out), new_state);
+          static_cast<const E*>(x), x_stride, static_cast<const E*>(gate), g_stride, state, rows * D, (int)D,
+          static_cast<E*>(out), new_state);
     });
   });
   SPK_LAUNCH_CHECK();

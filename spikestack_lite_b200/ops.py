@@ -767,12 +767,20 @@ def gated_recurrence(x, gate, state=None, form="leaky", dim=-2, lengths=None):
     return _recurrence_forward(x, gate, state, form, dim, lengths, False)[:2]
 
 
+def _rows(t):
+    """t, or a contiguous copy, as rows of its last dimension, and their stride."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    st = _time_strides(t.unsqueeze(-2), t.dim() - 1)  # a time dimension of one step: the batch is the rows
+    return (t, st[0]) if st is not None else (t.contiguous(), t.shape[-1])
+
+
 def gated_recurrence_step(x, gate, state, form="leaky", new_state=None):
     """One step of gated_recurrence for streaming: x and gate [..., d] of one
     time step, state float32 of the same shape -> (h, new state): h in x's
     dtype, the state in float32.  ``new_state``: the tensor to write it to
-    (contiguous float32; `state` itself updates it in place).  Not
-    differentiable."""
+    (contiguous float32; `state` itself updates it in place).  x and gate may be
+    slices whose last dimension is contiguous.  Not differentiable."""
     what = "gated_recurrence_step"
     dt = _checked(what, x, gate, state, new_state)
     form = _form(form, what)
@@ -786,9 +794,13 @@ def gated_recurrence_step(x, gate, state, form="leaky", new_state=None):
         new_state = torch.empty_like(x, dtype=torch.float32, memory_format=torch.contiguous_format)
     elif new_state.dtype != torch.float32 or new_state.shape != x.shape or not new_state.is_contiguous():
         raise EngineError(f"{what}: new_state must be contiguous float32 of x's shape {tuple(x.shape)}")
-    x, gate, state = _contig(x), _contig(gate), _contig(state)
-    out = torch.empty_like(x)
-    _call(x, "spk_recurrence_step", ptr(x), ptr(gate), dt, form, x.numel(), ptr(state), ptr(out), ptr(new_state))
+    if x.dim() == 0:
+        raise EngineError(f"{what}: x must have a channel dimension")
+    D = x.shape[-1]
+    (x, xs), (gate, gs), state = _rows(x), _rows(gate), _contig(state)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _call(x, "spk_recurrence_step", ptr(x), xs, ptr(gate), gs, dt, form, x.numel() // D if D else 0, D, ptr(state),
+          ptr(out), ptr(new_state))
     return out, new_state
 
 

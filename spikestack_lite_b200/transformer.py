@@ -12,7 +12,9 @@ Not mirrored (outside the forward hot path): the conv and text stems
 (``use_conv_stem``, ``text_vocab`` raise), ``forward_text`` and the
 exact-SNN latency loss; with ``use_exact=True`` the head's parameters exist
 (for state-dict compatibility) but, as in the reference, forward() does not
-use them.
+use them.  Beyond the reference: ``dropout`` (counter-based, on the blocks'
+branches in training mode) and ``use_recurrence`` (a GatedRecurrence over the
+planes behind the blocks).
 """
 import torch
 import torch.nn as nn
@@ -21,6 +23,7 @@ from . import ops
 from ._lib import EngineError
 from .attention import AstrocyteHebbianBlock, spike_fn
 from .gsmc import FusedGSMC
+from .recurrence import GatedRecurrence
 
 
 class SpireEncoder(nn.Module):
@@ -71,7 +74,8 @@ class SpikingTransformer(nn.Module):
                  num_layers=1, n_repeats=3, use_spikeskip=False, expansion=None, spike_readout=True,
                  temporal=False, spike_threshold=0.0, use_gsmc=False, gsmc_pool="mean", gsmc_readout=False,
                  use_exact=False, exact_weight=1.0, exact_beta_init=1.0, exact_beta_end=8.0,
-                 use_conv_stem=False, conv_kernels=32, text_vocab=None, padding_idx=0):
+                 use_conv_stem=False, conv_kernels=32, text_vocab=None, padding_idx=0, dropout=0.0,
+                 use_recurrence=False):
         super().__init__()
         if use_conv_stem or text_vocab is not None:
             raise EngineError("SpikingTransformer: the conv and text stems are not part of this engine")
@@ -85,7 +89,7 @@ class SpikingTransformer(nn.Module):
             expansion = 8 if use_spikeskip else 4  # models/transformer.py:93-96 (engine present)
         self.blocks = nn.ModuleList([
             AstrocyteHebbianBlock(d_model=d_model, num_heads=num_heads, expansion=expansion, v_levels=v_levels,
-                                  use_spikeskip=use_spikeskip, spike_threshold=spike_threshold)
+                                  use_spikeskip=use_spikeskip, spike_threshold=spike_threshold, dropout=dropout)
             for _ in range(num_layers)
         ])
         self.gsmc = None
@@ -99,6 +103,11 @@ class SpikingTransformer(nn.Module):
         self.classifier = nn.Linear(d_model, num_classes)
         self.exact_head = _LatencyHeadParams(d_model, num_classes) if self.use_exact else None
         self.exact_weight = float(exact_weight)
+        self.recurrence = None  # created last: a seed gives the other parameters with or without it
+        if use_recurrence:
+            if not self.temporal:
+                raise ValueError("use_recurrence=True requires temporal=True (it runs over the Spire T-planes).")
+            self.recurrence = GatedRecurrence(d_model, dropout=dropout)
 
     def load_reference_state_dict(self, sd, strict=True):
         """Load a reference state dict; maps fc2.* <-> fc2.linear.* between the
@@ -132,6 +141,8 @@ class SpikingTransformer(nn.Module):
         for i, block in enumerate(self.blocks):
             nxt = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else None
             context, context_norm = block.forward_fused(context, context_norm, nxt)
+        if self.recurrence is not None:
+            context = self.recurrence(context)[0]
         if self.gsmc is not None:
             context = self.gsmc(context, T=context.shape[0])
         pooled_over_time = self.temporal and self.gsmc is None

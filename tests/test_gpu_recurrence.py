@@ -172,6 +172,12 @@ def test_steps_follow_the_recurrence(form, dtype):
         out2, same = ops.gated_recurrence_step(x[:, t].cuda(), gate[:, t].cuda(), s, form=form, new_state=s)
         assert same is s and torch.equal(out, out2) and torch.equal(s, new)
     assert_within(s, ref.last, ref.last_err, "state")
+    # halves of one projection, and every other row of a larger tensor
+    both = torch.cat([x[:, 0], gate[:, 0]], -1).cuda()
+    want = ops.gated_recurrence_step(x[:, 0].cuda(), gate[:, 0].cuda(), state.cuda(), form=form)
+    for xs, gs in ((both[:, :37], both[:, 37:]), (x.cuda()[:, 0], gate.cuda()[:, 0])):
+        got = ops.gated_recurrence_step(xs, gs, state.cuda(), form=form)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     # split in two calls through the state
     a = ops.gated_recurrence(x[:, :4].cuda(), gate[:, :4].cuda(), state.cuda(), form=form)
     b = ops.gated_recurrence(x[:, 4:].cuda(), gate[:, 4:].cuda(), a[1], form=form)

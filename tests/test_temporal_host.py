@@ -94,12 +94,12 @@ def test_recurrence_entry_points_reject_bad_arguments(lib):
         assert bwd(**bad) == SPK_EINVAL, bad
     assert b"carry" in lib.spk_last_error()
 
-    def step(x=P, gate=P, dtype=0, form=1, n=4, state=P, out=P, new=P):
-        return lib.spk_recurrence_step(x, gate, dtype, form, n, state, out, new, None)
+    def step(x=P, gate=P, dtype=0, form=1, rows=4, D=8, state=P, out=P, new=P):
+        return lib.spk_recurrence_step(x, 8, gate, 8, dtype, form, rows, D, state, out, new, None)
 
-    assert step(n=0) == SPK_OK
-    for bad in (dict(n=-1), dict(x=None), dict(state=None), dict(out=None), dict(new=None), dict(dtype=9),
-                dict(form=7), dict(new=ODD)):
+    assert step(rows=0) == SPK_OK and step(D=0) == SPK_OK
+    for bad in (dict(rows=-1), dict(D=-1), dict(x=None), dict(state=None), dict(out=None), dict(new=None),
+                dict(dtype=9), dict(form=7), dict(new=ODD), dict(rows=1 << 40, D=1 << 20)):
         assert step(**bad) == SPK_EINVAL, bad
 
 
@@ -170,3 +170,35 @@ def test_time_strides():
     assert _time_strides(x[0, 0, 0].expand(3, 5, 8), 1) == (0, 0)
     t, st = _time_major(x, 1)
     assert t.shape == x.shape and st == _time_strides(t, 1) == (24, 8)
+
+
+def test_modules_on_the_host():
+    from spikestack_lite_b200._lib import EngineError
+    from spikestack_lite_b200.recurrence import Dropout, GatedRecurrence
+    from spikestack_lite_b200.transformer import SpikingTransformer
+
+    cfg = dict(temporal=True, n_repeats=3, use_spikeskip=True, expansion=4)
+    torch.manual_seed(0)
+    plain = SpikingTransformer(**cfg).state_dict()
+    torch.manual_seed(0)
+    more = SpikingTransformer(**cfg, use_recurrence=True).state_dict()
+    assert all(torch.equal(more[k], v) for k, v in plain.items())  # a seed's weights do not change
+    assert {k.split(".")[0] for k in set(more) - set(plain)} == {"recurrence"}
+    assert set(SpikingTransformer(**cfg, dropout=0.1).state_dict()) == set(plain)  # no mask, no key
+    with pytest.raises(ValueError):
+        SpikingTransformer(use_recurrence=True)
+    with pytest.raises(ValueError):
+        GatedRecurrence(10, groups=4)
+    with pytest.raises(ValueError):
+        Dropout(1.5)
+    m = GatedRecurrence(16, groups=4)
+    with pytest.raises(EngineError, match="CUDA"):
+        m(torch.zeros(3, 2, 5, 16))
+    with pytest.raises(EngineError, match="CUDA"):
+        m.step(torch.zeros(2, 5, 16))
+    d = Dropout(0.5)
+    d.manual_seed(7, 3)
+    assert d.key.tolist() == [7, 3]
+    d.eval()
+    x = torch.randn(4)
+    assert d(x) is x and torch.equal(d(x, residual=x), x + x) and d.key.tolist() == [7, 3]
