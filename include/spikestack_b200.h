@@ -363,7 +363,7 @@ int spk_recurrence_step(const void* x, int64_t x_stride, const void* gate, int64
  * z = (x - mean) rstd weight[c] + bias[c], Y = act(z).  X and Y hold dtype;
  * weight, bias (null: 1, 0), mean and rstd [S, G] (outputs, both or neither
  * null) are fp32.  No reference counterpart (its blocks use layer norm). */
-size_t spk_group_norm_workspace_bytes(int64_t S, int64_t P, int C, int G);
+size_t spk_group_norm_workspace_bytes(int dtype, int64_t S, int64_t P, int C, int G);
 int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P, int C, int G, const float* weight,
                        const float* bias, float eps, int act, float thr, void* Y, float* mean, float* rstd,
                        void* workspace, size_t workspace_bytes, spk_stream_t stream);

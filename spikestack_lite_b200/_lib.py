@@ -66,7 +66,7 @@ SIGNATURES = {
     "spk_recurrence_backward": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P,
                                      _L, _L, _P, _P]),
     "spk_recurrence_step": (_I, [_P, _L, _P, _L, _I, _I, _L, _L, _P, _P, _P, _P]),
-    "spk_group_norm_workspace_bytes": (_Z, [_L, _L, _I, _I]),
+    "spk_group_norm_workspace_bytes": (_Z, [_I, _L, _L, _I, _I]),
     "spk_group_norm_act": (_I, [_P, _I, _L, _L, _I, _I, _P, _P, _F, _I, _F, _P, _P, _P, _P, _Z, _P]),
     "spk_group_norm_act_backward": (_I, [_P, _P, _I, _L, _L, _I, _I, _P, _P, _P, _P, _I, _F, _P, _P, _P, _P, _Z, _P]),
     "spk_dropout": (_I, [_P, _P, _I, _L, _c.c_double, _c.c_uint64, _c.c_uint64, _P, _P, _P]),

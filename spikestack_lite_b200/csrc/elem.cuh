@@ -87,6 +87,24 @@ __device__ __forceinline__ float rcp_fast(float x) {
 __device__ __forceinline__ void grid_dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// The two halves of a cluster's barrier, and a value in another block's shared
+// memory (the address of this block's copy of it).
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 cluster_load(const float2* mine, uint32_t rank) {
+  uint32_t there;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(there) : "memory");
+  return v;
+}
+
 inline size_t elem_bytes(int dtype) { return dtype == SPK_F32 ? 4 : (dtype == SPK_BF16 || dtype == SPK_F16) ? 2 : 0; }
 
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

@@ -31,7 +31,8 @@ struct GnArgs {
   int64_t S, P;
   int C, G, cg;
   int tpr, rpp, threads;  // threads side by side and rows at once in a block
-  int k, rows, tiles;   // groups per block (resident); positions per tile (tiled); blocks per sample
+  int held, split;      // bytes of the tensors that a block holds, blocks per sample and groups (resident)
+  int k, rows, tiles;   // groups per block (resident); positions per block; blocks per sample (and position share)
   int64_t parts;        // rows of `part`
   float eps, thr;
 };
@@ -166,118 +167,173 @@ __device__ __forceinline__ Pack<E, V> gn_backward(const Pack<E, V>& x, const Pac
   return pack_f32<E, V>(o);
 }
 
-// ---- resident form: a block holds a sample's k groups (all positions) in
-// registers, so x (and gy) cross HBM once.  N packs of 16 bytes per thread.
-template <int N>
-__device__ __forceinline__ int gn_rows(const GnArgs& a, const GnSpot& q) {  // rows of this thread, at most N
-  return q.live ? (int)ceil_div(max64(a.P - q.r, 0), a.rpp) : 0;
-}
+// ---- resident form: a block, or a cluster of `split` blocks with a share of
+// the positions each, holds a sample's k groups in shared memory, so x (and gy)
+// cross HBM once.  Every thread copies the packs (16 bytes) that it will read
+// itself; what waits is memory, not registers, so some 30 warps share an SM.
+// The blocks of a cluster read each other's group sums, in the order of ranks.
+struct GnShare {
+  int64_t s, p0;  // sample, first position
+  int P, rank;    // positions
+  int g0, ng;     // groups
 
-template <typename E, int N, int V>
-__device__ __forceinline__ void gn_load(const E* p, int64_t step, int rows, Pack<E, V>* v) {
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < rows) v[i] = load_pack<E, V>(p + i * step);
-}
+  __device__ __forceinline__ explicit GnShare(const GnArgs& a) {
+    const int64_t unit = (int64_t)blockIdx.x / a.split;
+    rank = (int)(blockIdx.x - unit * a.split);
+    s = unit / a.tiles;
+    g0 = (int)(unit - s * a.tiles) * a.k;
+    ng = min(a.k, a.G - g0);
+    p0 = (int64_t)rank * a.rows;
+    P = positions(a, rank);
+  }
+  __device__ __forceinline__ static int positions(const GnArgs& a, int rank) {
+    return (int)max64(min64(a.P - (int64_t)rank * a.rows, a.rows), 0);
+  }
+};
 
-// Mean and sum of squares about it of `rows` packs' channels j0 .. j0 + J - 1.
-template <typename E, int N, int V, int J>
-__device__ __forceinline__ float4 gn_moments(const Pack<E, V>* x, int rows, int j0) {
-  const float n = (float)(rows * J), inv = rows > 0 ? __fdividef(1.0f, n) : 0.0f;
-  float sum = 0.0f, m2 = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < rows) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) sum += elem_to_f32(x[i].e[j0 + j]);
-    }
-  const float mean = sum * inv;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < rows) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const float d = elem_to_f32(x[i].e[j0 + j]) - mean;
-        m2 = fmaf(d, d, m2);
-      }
-    }
-  return make_float4(mean, m2, n, 0.0f);
-}
+template <typename E, int V>
+struct GnPacks {
+  E* slot;  // the thread's packs of one tensor, blockDim packs apart
+  int rows;
 
-// WHOLE: every pack lies in one group (cg is a multiple of V).
-template <typename E, int ACT, int N, bool WHOLE>
-__global__ void __launch_bounds__(kGnThreads, N > 4 ? 2 : 4) gn_resident_kernel(GnArgs a) {
+  __device__ __forceinline__ GnPacks(unsigned char* smem, int rows_)
+      : slot(reinterpret_cast<E*>(smem) + threadIdx.x * V), rows(rows_) {}
+  __device__ __forceinline__ void ask(const E* p, int64_t step) const {
+    E* to = slot;
+    for (int i = 0; i < rows; ++i, p += step, to += blockDim.x * V)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(p) : "memory");
+  }
+  __device__ __forceinline__ Pack<E, V> get(int i) const { return load_pack<E, V>(slot + (size_t)i * blockDim.x * V); }
+};
+__device__ __forceinline__ void gn_wait_packs() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// WHOLE: every pack lies in one group (cg is a multiple of V); a part is then
+// the moments of one thread, else those of one channel of one thread.
+template <typename E, int ACT, bool WHOLE>
+__global__ void __launch_bounds__(512, 2) gn_resident_kernel(GnArgs a) {
   constexpr int V = 16 / (int)sizeof(E), M = WHOLE ? 1 : V;
   extern __shared__ __align__(16) unsigned char gn_smem[];
-  float4* const part = reinterpret_cast<float4*>(gn_smem);  // [groups][parts] mean, sum of squares about it, count
-  const int64_t s = blockIdx.x / a.tiles;
-  const int g0 = (int)(blockIdx.x - s * a.tiles) * a.k, ng = min(a.k, a.G - g0), width = ng * a.cg;
+  const GnShare h(a);
+  const int width = h.ng * a.cg;
   GnSpot q = gn_spot(V, a.tpr, a.rpp);
   q.live = q.live && q.cv < width;
-  const int rows = gn_rows<N>(a, q), c0 = g0 * a.cg + q.cv;
-  const int64_t at = (s * a.P + q.r) * a.C + c0, step = (int64_t)a.rpp * a.C;
-  Pack<E, V> x[N];
-  gn_load<E, N, V>(static_cast<const E*>(a.x) + at, step, rows, x);
-  const int per_row = WHOLE ? a.cg / V : a.cg, parts = a.rpp * per_row;  // of one group
+  const int least = h.P / a.rpp, extra = h.P - least * a.rpp;
+  const int rows = q.live ? least + (q.r < extra ? 1 : 0) : 0, c0 = h.g0 * a.cg + q.cv;
+  const int64_t at = (h.s * a.P + h.p0 + q.r) * a.C + c0, step = (int64_t)a.rpp * a.C;
+  const GnPacks<E, V> x(gn_smem, rows);
+  x.ask(static_cast<const E*>(a.x) + at, step);
+  float2* const part = reinterpret_cast<float2*>(gn_smem + a.held);  // [groups][parts] mean, sum of squares about it
+  const int per_row = WHOLE ? a.cg / V : a.cg, parts = a.rpp * per_row;  // of one group, row by row
+  float2* const stat = part + a.k * parts;                              // [k]
+  gn_wait_packs();
   if (q.live) {
-    if (WHOLE) {
-      const int g = q.cv / a.cg;
-      part[g * parts + q.r * per_row + (q.cv - g * a.cg) / V] = gn_moments<E, N, V, V>(x, rows, 0);
-    } else {
+    float sum[M], m2[M];
+#pragma unroll
+    for (int j = 0; j < M; ++j) sum[j] = m2[j] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < rows; ++i) {
+      const Pack<E, V> p = x.get(i);
+      float all = 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int g = (q.cv + j) / a.cg;
-        part[g * parts + q.r * per_row + (q.cv + j - g * a.cg)] = gn_moments<E, N, V, 1>(x, rows, j);
+        if (M > 1)
+          sum[M > 1 ? j : 0] += elem_to_f32(p.e[j]);
+        else
+          all += elem_to_f32(p.e[j]);
       }
+      if (M == 1) sum[0] += all;
     }
-  }
-  __syncthreads();
-  // one warp per group
-  const int lane = threadIdx.x & 31;
-  const float total = (float)a.P * (float)a.cg;
-  float2* const stat = reinterpret_cast<float2*>(part + a.k * parts);  // [k]
-  for (int g = threadIdx.x >> 5; g < ng; g += kGnThreads / 32) {
-    float sum = 0.0f, m2 = 0.0f;
-    for (int i = lane; i < parts; i += 32) {
-      const float4 v = part[g * parts + i];
-      sum = fmaf(v.z, v.x, sum);
-    }
-    const float mean = gn_warp_sum(sum) / total;
-    for (int i = lane; i < parts; i += 32) {
-      const float4 v = part[g * parts + i];
-      const float d = v.x - mean;
-      m2 += fmaf(v.z * d, d, v.y);
-    }
-    const float rstd = rsqrtf(gn_warp_sum(m2) / total + a.eps);
-    if (lane == 0) {
-      stat[g] = make_float2(mean, rstd);
-      if (a.mean != nullptr) {
-        a.mean[s * a.G + g0 + g] = mean;
-        a.rstd[s * a.G + g0 + g] = rstd;
-      }
-    }
-  }
-  __syncthreads();
-  if (!q.live) return;
-  GnAffine<V, M> f;
-  gn_groups<V, M>(q.cv, a.cg, [&](int j, int g) {
-    if (M > 1 || j == 0) {
-      f.mean[M > 1 ? j : 0] = stat[g].x;
-      f.rstd[M > 1 ? j : 0] = stat[g].y;
-    }
-  });
-  gn_affine<V, M>(a, c0, &f);
-  E* const y = static_cast<E*>(a.y) + at;
+    const float inv = rows > 0 ? __fdividef(1.0f, (float)(rows * (WHOLE ? V : 1))) : 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < rows) store_pack<E, V>(y + i * step, gn_forward<E, ACT, V, M>(x[i], f, a.thr));
+    for (int j = 0; j < M; ++j) sum[j] *= inv;
+#pragma unroll 4
+    for (int i = 0; i < rows; ++i) {
+      const Pack<E, V> p = x.get(i);
+      float all = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = elem_to_f32(p.e[j]) - sum[M > 1 ? j : 0];
+        if (M > 1)
+          m2[M > 1 ? j : 0] = fmaf(d, d, m2[M > 1 ? j : 0]);
+        else
+          all = fmaf(d, d, all);
+      }
+      if (M == 1) m2[0] += all;
+    }
+    gn_groups<V, M>(q.cv, a.cg, [&](int j, int g) {
+      if (M > 1 || j == 0)
+        part[g * parts + q.r * per_row + (q.cv + j - g * a.cg) / (WHOLE ? V : 1)] =
+            make_float2(sum[M > 1 ? j : 0], m2[M > 1 ? j : 0]);
+    });
+  }
+  __syncthreads();
+  // one warp per group; the first `more` parts have a row more than the rest
+  const int lane = threadIdx.x & 31, more = extra * per_row;
+  const float mine = (float)h.P * (float)a.cg, total = (float)a.P * (float)a.cg;
+  const float n_more = (float)((least + 1) * (WHOLE ? V : 1)), n_less = (float)(least * (WHOLE ? V : 1));
+  for (int g = threadIdx.x >> 5; g < h.ng; g += blockDim.x / 32) {
+    float sum = 0.0f, m2 = 0.0f;
+    for (int i = lane; i < parts; i += 32) sum = fmaf(i < more ? n_more : n_less, part[g * parts + i].x, sum);
+    const float mean = h.P > 0 ? gn_warp_sum(sum) / mine : 0.0f;
+    for (int i = lane; i < parts; i += 32) {
+      const float2 v = part[g * parts + i];
+      const float d = v.x - mean;
+      m2 += fmaf((i < more ? n_more : n_less) * d, d, v.y);
+    }
+    m2 = gn_warp_sum(m2);
+    if (lane == 0) stat[g] = make_float2(mean, m2);
+  }
+  float2* const own = stat + a.k;  // [k] mean and rstd
+  if (a.split > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  for (int g = threadIdx.x; g < h.ng; g += blockDim.x) {
+    float2 m = stat[g];
+    if (a.split > 1) {
+      float sum = 0.0f, m2 = 0.0f;
+      for (int r = 0; r < a.split; ++r)
+        sum = fmaf((float)GnShare::positions(a, r) * (float)a.cg, cluster_load(stat + g, r).x, sum);
+      const float mean = sum / total;
+      for (int r = 0; r < a.split; ++r) {
+        const float2 v = cluster_load(stat + g, r);
+        const float d = v.x - mean;
+        m2 += fmaf((float)GnShare::positions(a, r) * (float)a.cg * d, d, v.y);
+      }
+      m = make_float2(mean, m2);
+    }
+    m.y = rsqrtf(m.y / total + a.eps);
+    own[g] = m;
+    if (a.mean != nullptr && h.rank == 0) {
+      a.mean[h.s * a.G + h.g0 + g] = m.x;
+      a.rstd[h.s * a.G + h.g0 + g] = m.y;
+    }
+  }
+  if (a.split > 1) cluster_arrive();
+  __syncthreads();
+  if (q.live) {
+    GnAffine<V, M> f;
+    gn_groups<V, M>(q.cv, a.cg, [&](int j, int g) {
+      if (M > 1 || j == 0) {
+        f.mean[M > 1 ? j : 0] = own[g].x;
+        f.rstd[M > 1 ? j : 0] = own[g].y;
+      }
+    });
+    gn_affine<V, M>(a, c0, &f);
+    E* y = static_cast<E*>(a.y) + at;
+#pragma unroll 2
+    for (int i = 0; i < rows; ++i, y += step) store_pack<E, V>(y, gn_forward<E, ACT, V, M>(x.get(i), f, a.thr));
+  }
+  if (a.split > 1) cluster_wait();  // stat is read by the others
 }
 
 // Sums over the rows of part [rpp][width], by the whole block and in a fixed
 // order: `some` [segments][width] (at most one entry per thread), then sums [width].
 __device__ __forceinline__ void gn_channel_sums(const float2* part, int rpp, int width, float2* some, float2* sums) {
-  const int segments = max(1, min(rpp, kGnThreads / width));
-  for (int i = threadIdx.x; i < segments * width; i += kGnThreads) {
+  const int threads = blockDim.x, segments = max(1, min(rpp, threads / width));
+  for (int i = threadIdx.x; i < segments * width; i += threads) {
     const int seg = i / width, c = i - seg * width;
     float2 v = make_float2(0.0f, 0.0f);
     for (int r = seg; r < rpp; r += segments) {
@@ -288,7 +344,7 @@ __device__ __forceinline__ void gn_channel_sums(const float2* part, int rpp, int
   }
   __syncthreads();
   if (segments > 1) {
-    for (int c = threadIdx.x; c < width; c += kGnThreads) {
+    for (int c = threadIdx.x; c < width; c += threads) {
       float2 v = some[c];
       for (int i = 1; i < segments; ++i) {
         v.x += some[i * width + c].x;
@@ -300,86 +356,95 @@ __device__ __forceinline__ void gn_channel_sums(const float2* part, int rpp, int
   }
 }
 
-template <typename E, int ACT, int N, bool WHOLE>
-__global__ void __launch_bounds__(kGnThreads, N > 2 ? 2 : 3) gn_resident_backward_kernel(GnArgs a) {
+template <typename E, int ACT, bool WHOLE>
+__global__ void __launch_bounds__(512, 2) gn_resident_backward_kernel(GnArgs a) {
   constexpr int V = 16 / (int)sizeof(E), M = WHOLE ? 1 : V;
   extern __shared__ __align__(16) unsigned char gn_smem[];
-  float2* const part = reinterpret_cast<float2*>(gn_smem);  // [rpp][width] sums of dz and dz xhat
   grid_dependents_may_start();
-  const int64_t s = blockIdx.x / a.tiles;
-  const int g0 = (int)(blockIdx.x - s * a.tiles) * a.k, ng = min(a.k, a.G - g0), width = ng * a.cg;
+  const GnShare h(a);
+  const int width = h.ng * a.cg;
   GnSpot q = gn_spot(V, a.tpr, a.rpp);
   q.live = q.live && q.cv < width;
-  const int rows = gn_rows<N>(a, q), c0 = g0 * a.cg + q.cv;
-  const int64_t at = (s * a.P + q.r) * a.C + c0, step = (int64_t)a.rpp * a.C;
-  Pack<E, V> x[N], gy[N];
-  gn_load<E, N, V>(static_cast<const E*>(a.x) + at, step, rows, x);
-  gn_load<E, N, V>(static_cast<const E*>(a.gy) + at, step, rows, gy);
+  const int rows = q.live ? (int)ceil_div(max(h.P - q.r, 0), a.rpp) : 0, c0 = h.g0 * a.cg + q.cv;
+  const int64_t at = (h.s * a.P + h.p0 + q.r) * a.C + c0, step = (int64_t)a.rpp * a.C;
+  const GnPacks<E, V> x(gn_smem, rows), gy(gn_smem + a.held / 2, rows);
+  x.ask(static_cast<const E*>(a.x) + at, step);
+  gy.ask(static_cast<const E*>(a.gy) + at, step);
+  float2* const part = reinterpret_cast<float2*>(gn_smem + a.held);  // [rpp][width] sums of dz and dz xhat
+  float2* const sums = part + a.rpp * a.k * a.cg;                    // [width]
+  float2* const coef = sums + a.k * a.cg;                            // [k]
   GnAffine<V, M> f;
-  constexpr bool kKeep = N <= 2;  // dz and x - mean stay in registers; with more rows they are computed again
-  float keep_dz[kKeep ? N : 1][V], keep_d[kKeep ? N : 1][V];
+  if (q.live) gn_affine<V, M>(a, h.s, c0, &f);
+  gn_wait_packs();
   if (q.live) {
-    gn_affine<V, M>(a, s, c0, &f);
+    float s1[V], s2[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float2 acc = make_float2(0.0f, 0.0f);
+    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
+#pragma unroll 2
+    for (int i = 0; i < rows; ++i) {
+      const Pack<E, V> xv = x.get(i), gv = gy.get(i);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < rows) {
-          float d;
-          const float dz = gn_dz<E, ACT, V, M>(x[i], gy[i], f, j, a.thr, &d);
-          if (kKeep) {
-            keep_dz[kKeep ? i : 0][j] = dz;
-            keep_d[kKeep ? i : 0][j] = d;
-          }
-          acc.x += dz;
-          acc.y = fmaf(dz, d, acc.y);
-        }
-      part[q.r * width + q.cv + j] = make_float2(acc.x, acc.y * f.rstd[M > 1 ? j : 0]);
+      for (int j = 0; j < V; ++j) {
+        float d;
+        const float dz = gn_dz<E, ACT, V, M>(xv, gv, f, j, a.thr, &d);
+        s1[j] += dz;
+        s2[j] = fmaf(dz, d, s2[j]);
+      }
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      part[q.r * width + q.cv + j] = make_float2(s1[j], s2[j] * f.rstd[M > 1 ? j : 0]);
   }
   __syncthreads();
-  float2* const sums = part + a.rpp * a.k * a.cg;  // [width]
-  float2* const coef = sums + a.k * a.cg;          // [k]
-  gn_channel_sums(part, a.rpp, width, coef + a.k, sums);
+  float2* const own = coef + a.k;  // [k] this block's sums of dn and dn xhat
+  gn_channel_sums(part, a.rpp, width, own + a.k, sums);
   const int lane = threadIdx.x & 31;
   const float inv = 1.0f / ((float)a.P * (float)a.cg);
-  for (int g = threadIdx.x >> 5; g < ng; g += kGnThreads / 32) {
+  for (int g = threadIdx.x >> 5; g < h.ng; g += blockDim.x / 32) {
     float s1 = 0.0f, s2 = 0.0f;
     for (int i = lane; i < a.cg; i += 32) {
-      const float w = a.weight != nullptr ? a.weight[(g0 + g) * a.cg + i] : 1.0f;
+      const float w = a.weight != nullptr ? a.weight[(h.g0 + g) * a.cg + i] : 1.0f;
       s1 = fmaf(w, sums[g * a.cg + i].x, s1);
       s2 = fmaf(w, sums[g * a.cg + i].y, s2);
     }
     s1 = gn_warp_sum(s1);
     s2 = gn_warp_sum(s2);
-    if (lane == 0) coef[g] = make_float2(s1 * inv, s2 * inv);
+    if (lane == 0) own[g] = make_float2(s1, s2);
   }
   if (a.part != nullptr)
-    for (int c = threadIdx.x; c < width; c += kGnThreads)
-      *reinterpret_cast<float2*>(a.part + (s * a.C + g0 * a.cg + c) * 2) = sums[c];
-  __syncthreads();
-  if (!q.live) return;
-  E* const dx = static_cast<E*>(a.y) + at;
-  float2 k[M];
-  gn_groups<V, M>(q.cv, a.cg, [&](int j, int g) {
-    if (M > 1 || j == 0) k[M > 1 ? j : 0] = gn_pull(coef[g], f.rstd[M > 1 ? j : 0]);
-  });
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < rows) {
-      if (kKeep) {
-        float o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float2 kj = k[M > 1 ? j : 0];
-          o[j] = fmaf(keep_dz[kKeep ? i : 0][j], f.a[j], fmaf(keep_d[kKeep ? i : 0][j], kj.y, kj.x));
-        }
-        store_pack<E, V>(dx + i * step, pack_f32<E, V>(o));
-      } else {
-        store_pack<E, V>(dx + i * step, gn_backward<E, ACT, V, M>(x[i], gy[i], f, k, a.thr));
+    for (int c = threadIdx.x; c < width; c += blockDim.x)
+      *reinterpret_cast<float2*>(a.part + ((h.s * a.split + h.rank) * a.C + h.g0 * a.cg + c) * 2) = sums[c];
+  if (a.split > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  for (int g = threadIdx.x; g < h.ng; g += blockDim.x) {
+    float2 m = own[g];
+    if (a.split > 1) {
+      m = make_float2(0.0f, 0.0f);
+      for (int r = 0; r < a.split; ++r) {
+        const float2 v = cluster_load(own + g, r);
+        m.x += v.x;
+        m.y += v.y;
       }
     }
+    coef[g] = make_float2(m.x * inv, m.y * inv);
+  }
+  if (a.split > 1) cluster_arrive();
+  __syncthreads();
+  if (q.live) {
+    E* dx = static_cast<E*>(a.y) + at;
+    float2 k[M];
+    gn_groups<V, M>(q.cv, a.cg, [&](int j, int g) {
+      if (M > 1 || j == 0) k[M > 1 ? j : 0] = gn_pull(coef[g], f.rstd[M > 1 ? j : 0]);
+    });
+#pragma unroll 2
+    for (int i = 0; i < rows; ++i, dx += step)
+      store_pack<E, V>(dx, gn_backward<E, ACT, V, M>(x.get(i), gy.get(i), f, k, a.thr));
+  }
+  if (a.split > 1) cluster_wait();  // own is read by the others
 }
 
 // ---- tiled form: samples larger than a block holds.  Tiles of `rows`
@@ -689,35 +754,63 @@ static int gn_vector(size_t eb, int C, const void* x, const void* gy, const void
   return 1;
 }
 
-// Resident form: the largest k groups per block whose positions fit into N
-// packs per thread and that leave enough blocks for the GPU; rows of at least
-// 64 bytes.  False: none (the sample is too large, or its rows do not divide
-// into packs).
-static bool gn_resident_plan(GnArgs* a, size_t eb, int V, int N) {
-  if (V != 16 / (int)eb) return false;
-  const int64_t unit = V / gn_gcd(a->cg, V);  // groups that make whole packs
-  for (int64_t k = ceil_div(a->G, unit) * unit; k >= 1; k -= unit) {
-    const int64_t kk = k > a->G ? a->G : k, width = kk * a->cg;
-    if (kk < a->G && (int64_t)(width * eb) < 64) return false;
-    if (width / V > kGnThreads) continue;
-    const int tpr = (int)(width / V), rpp = kGnThreads / tpr;
-    if (ceil_div(a->P, rpp) > N) continue;
-    const int64_t smaller = kk > unit ? (kk - 1) / unit * unit : kk;
-    if (a->S * ceil_div(a->G, kk) < 2 * 148 && smaller < kk && (int64_t)(smaller * a->cg * eb) >= 64) continue;
-    a->k = (int)kk;
-    a->tpr = tpr;
-    a->rpp = rpp;
-    a->tiles = (int)ceil_div(a->G, kk);
-    a->parts = a->S;
-    return a->S * a->tiles < (1ll << 31);
-  }
-  return false;
+// The resident form with k groups and T threads per block in clusters of
+// `split`; the shared memory of a block in bytes, 0 when it is above `most`.
+static size_t gn_resident_layout(GnArgs* a, int V, int k, int T, int split, bool backward, size_t most) {
+  const int64_t width = (int64_t)k * a->cg;
+  if (width % V != 0 || width / V > T) return 0;
+  a->k = k;
+  a->tpr = (int)(width / V);
+  a->rpp = T / a->tpr;
+  a->threads = T;
+  a->split = split;
+  a->tiles = (int)ceil_div(a->G, k);
+  a->rows = (int)ceil_div(a->P, split);
+  a->parts = a->S * split;
+  const double held = (double)ceil_div(a->rows, a->rpp) * T * 16 * (backward ? 2 : 1);
+  if (held > most) return 0;
+  a->held = (int)held;
+  const int parts = a->rpp * (int)width;
+  const size_t rest = backward ? (size_t)parts + width + 2 * k + T : (size_t)parts / (a->cg % V == 0 ? V : 1) + 2 * k;
+  const size_t smem = a->held + rest * sizeof(float2);
+  return smem <= most ? smem : 0;
 }
 
-static size_t gn_resident_smem(const GnArgs& a, int V, bool whole, bool backward) {
-  const size_t width = (size_t)a.k * a.cg;
-  if (backward) return (width * a.rpp + width + a.k + kGnThreads) * sizeof(float2);
-  return width / (whole ? V : 1) * a.rpp * sizeof(float4) + a.k * sizeof(float2);
+// Groups per block, threads and blocks per cluster: rows of at least 64 bytes
+// (or whole ones); the fewest blocks per cluster with which three blocks of 256
+// threads share an SM, else two of 512; then the most groups that leave enough
+// blocks for the GPU.  0: none (the sample is too large, or its rows do not
+// divide into packs).
+static size_t gn_resident_plan(GnArgs* a, size_t eb, int V, bool backward) {
+  if (V != 16 / (int)eb || a->S >= (1ll << 31) / ((int64_t)a->G * 8)) return 0;
+  const int64_t unit = V / gn_gcd(a->cg, V);  // groups that make whole packs
+  for (int T : {256, 512}) {
+    const size_t most = T == 256 ? 74 * 1024 : 112 * 1024;
+    for (int split = 1; split <= 8; split *= 2) {
+      int64_t best = 0;
+      for (int64_t n = ceil_div(a->G, unit); n >= 1; --n) {
+        const int64_t k = min64(n * unit, a->G);
+        if (k < a->G && k * a->cg * (int64_t)eb < 64) break;
+        if (gn_resident_layout(a, V, (int)k, T, split, backward, most) == 0) continue;
+        best = k;
+        if (a->S * a->tiles * split >= 2 * 148) break;
+      }
+      if (best > 0) return gn_resident_layout(a, V, (int)best, T, split, backward, most);
+    }
+  }
+  return 0;
+}
+
+template <typename K>
+static cudaError_t gn_launch_resident(K* kernel, const GnArgs& a, size_t smem, cudaStream_t st) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  const dim3 grid((unsigned)(a.S * a.tiles * a.split)), block((unsigned)a.threads);
+  if (a.split > 1) return launch_dependent_cluster(kernel, grid, block, smem, st, (unsigned)a.split, false, a);
+  kernel<<<grid, block, smem, st>>>(a);
+  return cudaGetLastError();
 }
 
 // Tiled form: blocks of up to 256 threads whose rows waste the fewest of them,
@@ -751,11 +844,22 @@ static void gn_tiled_plan(GnArgs* a, int V, int per_sm) {
   a->parts = a->S * a->tiles;
 }
 
-static size_t gn_part_bytes(int64_t S, int64_t P, int C) {
+// Bytes of the partial sums: of the tiled form, and of the resident backward
+// pass where that is used.
+static size_t gn_part_bytes(size_t eb, int64_t S, int64_t P, int C, int G) {
   int rows, tiles = 0, fewer;
   gn_tiled_rows(S, P, 4, &rows, &tiles);
   gn_tiled_rows(S, P, 3, &rows, &fewer);
-  return align_up((size_t)S * (tiles > fewer ? tiles : fewer) * C * 2 * sizeof(float), 256);
+  GnArgs a{};
+  a.S = S;
+  a.P = P;
+  a.C = C;
+  a.G = G;
+  a.cg = C / G;
+  const int wide = 16 / (int)eb;
+  const int split = C % wide == 0 && gn_resident_plan(&a, eb, wide, true) ? a.split : 1;
+  const int most = tiles > fewer ? tiles : fewer;
+  return align_up((size_t)S * (most > split ? most : split) * C * 2 * sizeof(float), 256);
 }
 
 static int gn_check(int dtype, int64_t S, int64_t P, int C, int G, int act, size_t* eb) {
@@ -800,9 +904,10 @@ inline void with_gn_act(int act, F&& f) {
 
 }  // namespace spk
 
-extern "C" size_t spk_group_norm_workspace_bytes(int64_t S, int64_t P, int C, int G) {
-  if (S <= 0 || P <= 0 || C <= 0 || G <= 0) return 0;
-  return spk::gn_part_bytes(S, P, C) + (size_t)S * G * 2 * sizeof(float);
+extern "C" size_t spk_group_norm_workspace_bytes(int dtype, int64_t S, int64_t P, int C, int G) {
+  const size_t eb = spk::elem_bytes(dtype);
+  if (eb == 0 || S <= 0 || P <= 0 || C <= 0 || G <= 0 || C % G != 0) return 0;
+  return spk::gn_part_bytes(eb, S, P, C, G) + (size_t)S * G * 2 * sizeof(float);
 }
 
 extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P, int C, int G, const float* weight,
@@ -817,9 +922,9 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
   SPK_REQUIRE(spk::aligned_to(X, eb) && spk::aligned_to(Y, eb) && spk::aligned_to(weight, 4) &&
                   spk::aligned_to(bias, 4) && spk::aligned_to(mean, 4) && spk::aligned_to(rstd, 4),
               "tensors must be aligned to their elements");
-  if (workspace == nullptr || workspace_bytes < spk_group_norm_workspace_bytes(S, P, C, G))
+  if (workspace == nullptr || workspace_bytes < spk_group_norm_workspace_bytes(dtype, S, P, C, G))
     return spk::fail(SPK_EWORKSPACE, "group norm needs a workspace of %zu bytes",
-                     spk_group_norm_workspace_bytes(S, P, C, G));
+                     spk_group_norm_workspace_bytes(dtype, S, P, C, G));
   SPK_REQUIRE(spk::aligned_to(workspace, 16), "the workspace must be 16-byte aligned");
   spk::GnArgs a{};
   a.x = X;
@@ -827,7 +932,7 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
   a.bias = bias;
   a.y = Y;
   a.part = static_cast<float*>(workspace);
-  float* tail = reinterpret_cast<float*>(static_cast<char*>(workspace) + spk::gn_part_bytes(S, P, C));
+  float* tail = reinterpret_cast<float*>(static_cast<char*>(workspace) + spk::gn_part_bytes(eb, S, P, C, G));
   a.mean = mean != nullptr ? mean : tail;
   a.rstd = rstd != nullptr ? rstd : tail + S * G;
   a.S = S;
@@ -839,28 +944,19 @@ extern "C" int spk_group_norm_act(const void* X, int dtype, int64_t S, int64_t P
   a.thr = thr;
   cudaStream_t st = (cudaStream_t)stream;
   const int V = spk::gn_vector(eb, C, X, nullptr, Y);
-  if (spk::gn_resident_plan(&a, eb, V, 4) || spk::gn_resident_plan(&a, eb, V, 16)) {
-    const bool whole = a.cg % V == 0;
-    const size_t smem = spk::gn_resident_smem(a, V, whole, false);
-    const bool few = spk::ceil_div(P, a.rpp) <= 4;
+  if (const size_t held = spk::gn_resident_plan(&a, eb, V, false)) {
+    cudaError_t rc = cudaSuccess;
     a.mean = mean;
     a.rstd = rstd;
     spk::with_elem(dtype, [&](auto e) {
       using E = decltype(e);
       spk::with_gn_act(act, [&](auto ac) {
         constexpr int ACT = decltype(ac)::value;
-        const unsigned grid = (unsigned)(S * a.tiles);
-        if (few && whole)
-          spk::gn_resident_kernel<E, ACT, 4, true><<<grid, spk::kGnThreads, smem, st>>>(a);
-        else if (few)
-          spk::gn_resident_kernel<E, ACT, 4, false><<<grid, spk::kGnThreads, smem, st>>>(a);
-        else if (whole)
-          spk::gn_resident_kernel<E, ACT, 16, true><<<grid, spk::kGnThreads, smem, st>>>(a);
-        else
-          spk::gn_resident_kernel<E, ACT, 16, false><<<grid, spk::kGnThreads, smem, st>>>(a);
+        rc = a.cg % V == 0 ? spk::gn_launch_resident(spk::gn_resident_kernel<E, ACT, true>, a, held, st)
+                           : spk::gn_launch_resident(spk::gn_resident_kernel<E, ACT, false>, a, held, st);
       });
     });
-    SPK_LAUNCH_CHECK();
+    SPK_CUDA_TRY(rc);
     spk::count_launch(1);
     return SPK_OK;
   }
@@ -910,9 +1006,9 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
                   spk::aligned_to(weight, 4) && spk::aligned_to(bias, 4) && spk::aligned_to(mean, 4) &&
                   spk::aligned_to(rstd, 4),
               "tensors must be aligned to their elements");
-  if (workspace == nullptr || workspace_bytes < spk_group_norm_workspace_bytes(S, P, C, G))
+  if (workspace == nullptr || workspace_bytes < spk_group_norm_workspace_bytes(dtype, S, P, C, G))
     return spk::fail(SPK_EWORKSPACE, "group norm needs a workspace of %zu bytes",
-                     spk_group_norm_workspace_bytes(S, P, C, G));
+                     spk_group_norm_workspace_bytes(dtype, S, P, C, G));
   SPK_REQUIRE(spk::aligned_to(workspace, 16), "the workspace must be 16-byte aligned");
   spk::GnArgs a{};
   a.x = X;
@@ -923,7 +1019,7 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
   a.mean = const_cast<float*>(mean);
   a.rstd = const_cast<float*>(rstd);
   a.part = static_cast<float*>(workspace);
-  a.coef = reinterpret_cast<float*>(static_cast<char*>(workspace) + spk::gn_part_bytes(S, P, C));
+  a.coef = reinterpret_cast<float*>(static_cast<char*>(workspace) + spk::gn_part_bytes(eb, S, P, C, G));
   a.dweight = dweight;
   a.dbias = dbias;
   a.S = S;
@@ -940,26 +1036,17 @@ extern "C" int spk_group_norm_act_backward(const void* X, const void* GY, int dt
     const cudaError_t e = spk::launch_dependent(kernel, grid, block, 0, st, a);
     if (rc == cudaSuccess) rc = e;
   };
-  if (spk::gn_resident_plan(&a, eb, V, 2) || spk::gn_resident_plan(&a, eb, V, 8)) {
-    const size_t smem = spk::gn_resident_smem(a, V, false, true);
-    const bool whole = a.cg % V == 0;
-    const bool few = spk::ceil_div(P, a.rpp) <= 2;
+  if (const size_t held = spk::gn_resident_plan(&a, eb, V, true)) {
     if (!params) a.part = nullptr;
     spk::with_elem(dtype, [&](auto e) {
       using E = decltype(e);
       spk::with_gn_act(act, [&](auto ac) {
         constexpr int ACT = decltype(ac)::value;
-        const unsigned grid = (unsigned)(S * a.tiles);
-        if (few && whole)
-          spk::gn_resident_backward_kernel<E, ACT, 2, true><<<grid, spk::kGnThreads, smem, st>>>(a);
-        else if (few)
-          spk::gn_resident_backward_kernel<E, ACT, 2, false><<<grid, spk::kGnThreads, smem, st>>>(a);
-        else if (whole)
-          spk::gn_resident_backward_kernel<E, ACT, 8, true><<<grid, spk::kGnThreads, smem, st>>>(a);
-        else
-          spk::gn_resident_backward_kernel<E, ACT, 8, false><<<grid, spk::kGnThreads, smem, st>>>(a);
+        rc = a.cg % V == 0 ? spk::gn_launch_resident(spk::gn_resident_backward_kernel<E, ACT, true>, a, held, st)
+                           : spk::gn_launch_resident(spk::gn_resident_backward_kernel<E, ACT, false>, a, held, st);
       });
     });
+    SPK_CUDA_TRY(rc);
     spk::count_launch(1);
   } else {
     spk::gn_tiled_plan(&a, V, 3);

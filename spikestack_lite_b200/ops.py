@@ -585,24 +585,35 @@ _DTYPES = {torch.float32: _lib.SPK_F32, torch.bfloat16: _lib.SPK_BF16, torch.flo
 def _checked(what, x, *others):
     """The dtype code of x, a CUDA tensor of one of the three types; the others
     (or None) on its device."""
-    if not (isinstance(x, torch.Tensor) and x.is_cuda):
-        require_cuda(x, what=what)
-    dev = x.get_device()
-    for t in others:
-        if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == dev):
-            require_cuda(t, what=what)
-            raise EngineError(f"{what}: tensors on {x.device} and {t.device}")
+    try:
+        dev = x.get_device() if x.is_cuda else -1
+        same = dev >= 0
+        for t in others:
+            if t is not None and t.get_device() != dev:
+                same = False
+    except AttributeError:
+        same = False
+    if not same:
+        require_cuda(x, *others, what=what)
+        if x is None:
+            raise EngineError(f"{what}: CUDA tensors required (this engine has no CPU path)")
+        raise EngineError(f"{what}: tensors on several devices")
     code = _DTYPES.get(x.dtype)
     if code is None:
         raise EngineError(f"{what}: float32, bfloat16 or float16 tensors required, got {x.dtype}")
     return code
 
 
+_ENTRY = {}
+
+
 def _call(t, name, *args):
     """Entry point `name` on t's device and its current stream (the last argument)."""
-    fn = getattr(_lib.load(), name)
+    fn = _ENTRY.get(name)
+    if fn is None:
+        fn = _ENTRY[name] = getattr(_lib.load(), name)
     dev = t.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
@@ -616,7 +627,11 @@ def _scratch(t, nbytes):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _backward(fn):
@@ -784,23 +799,25 @@ def gated_recurrence_step(x, gate, state, form="leaky", new_state=None):
     what = "gated_recurrence_step"
     dt = _checked(what, x, gate, state, new_state)
     form = _form(form, what)
-    if gate.dtype != x.dtype or gate.shape != x.shape:
+    shape = x.shape
+    if gate.dtype != x.dtype or gate.shape != shape:
         raise EngineError(f"{what}: gate must have x's shape and dtype")
-    if state.dtype != torch.float32 or state.shape != x.shape:
-        raise EngineError(f"{what}: state must be float32 of x's shape {tuple(x.shape)}")
+    if state.dtype != torch.float32 or state.shape != shape:
+        raise EngineError(f"{what}: state must be float32 of x's shape {tuple(shape)}")
     if _wants_grad(x, gate, state):
         raise EngineError(f"{what}: no backward pass (use gated_recurrence, or torch.no_grad())")
-    if new_state is None:
-        new_state = torch.empty_like(x, dtype=torch.float32, memory_format=torch.contiguous_format)
-    elif new_state.dtype != torch.float32 or new_state.shape != x.shape or not new_state.is_contiguous():
-        raise EngineError(f"{what}: new_state must be contiguous float32 of x's shape {tuple(x.shape)}")
-    if x.dim() == 0:
+    if not shape:
         raise EngineError(f"{what}: x must have a channel dimension")
-    D = x.shape[-1]
+    if new_state is not None and (new_state.dtype != torch.float32 or new_state.shape != shape
+                                  or not new_state.is_contiguous()):
+        raise EngineError(f"{what}: new_state must be contiguous float32 of x's shape {tuple(shape)}")
+    D = shape[-1]
     (x, xs), (gate, gs), state = _rows(x), _rows(gate), _contig(state)
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    _call(x, "spk_recurrence_step", ptr(x), xs, ptr(gate), gs, dt, form, x.numel() // D if D else 0, D, ptr(state),
-          ptr(out), ptr(new_state))
+    if new_state is None:
+        new_state = torch.empty_like(state)
+    _call(x, "spk_recurrence_step", x.data_ptr(), xs, gate.data_ptr(), gs, dt, form, x.numel() // D if D else 0, D,
+          state.data_ptr(), out.data_ptr(), new_state.data_ptr())
     return out, new_state
 
 
@@ -815,7 +832,7 @@ def _group_norm_forward(x, groups, weight, bias, eps, act, thr, keep):
     P = x.numel() // (S * C) if S else 0
     y = torch.empty_like(x)
     mean, rstd = x.new_empty(2, S, groups, dtype=torch.float32) if keep else (None, None)
-    ws = _scratch(x, lib.spk_group_norm_workspace_bytes(S, P, C, groups))
+    ws = _scratch(x, lib.spk_group_norm_workspace_bytes(_DTYPES[x.dtype], S, P, C, groups))
     _call(x, "spk_group_norm_act", ptr(x), _DTYPES[x.dtype], S, P, C, groups, ptr(weight), ptr(bias), eps, act, thr,
           ptr(y), ptr(mean), ptr(rstd), ptr(ws), 0 if ws is None else ws.numel())
     return y, mean, rstd
@@ -839,7 +856,7 @@ class _GroupNormAct(torch.autograd.Function):
         dx = torch.empty_like(x)
         dweight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         dbias = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
-        ws = _scratch(x, lib.spk_group_norm_workspace_bytes(S, P, C, ctx.groups))
+        ws = _scratch(x, lib.spk_group_norm_workspace_bytes(_DTYPES[x.dtype], S, P, C, ctx.groups))
         _call(x, "spk_group_norm_act_backward", ptr(x), ptr(gy), _DTYPES[x.dtype], S, P, C, ctx.groups, ptr(weight),
               ptr(bias), ptr(mean), ptr(rstd), ctx.act, ctx.thr, ptr(dx), ptr(dweight), ptr(dbias), ptr(ws),
               0 if ws is None else ws.numel())

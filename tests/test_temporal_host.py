@@ -106,8 +106,8 @@ def test_recurrence_entry_points_reject_bad_arguments(lib):
 def test_group_norm_entry_points_reject_bad_arguments(lib):
     from spikestack_lite_b200._lib import SPK_EINVAL, SPK_EWORKSPACE, SPK_OK
 
-    need = lib.spk_group_norm_workspace_bytes(2, 64, 32, 4)
-    assert need > 0 and lib.spk_group_norm_workspace_bytes(0, 64, 32, 4) == 0
+    need = lib.spk_group_norm_workspace_bytes(0, 2, 64, 32, 4)
+    assert need > 0 and lib.spk_group_norm_workspace_bytes(0, 0, 64, 32, 4) == 0
 
     def fwd(X=P, dtype=0, S=2, Pn=64, C=32, G=4, w=None, b=None, eps=1e-5, act=0, Y=P, mean=None, rstd=None, ws=P,
             n=need):
