@@ -780,13 +780,14 @@ static size_t gn_resident_layout(GnArgs* a, int V, int k, int T, int split, bool
 // (or whole ones); the fewest blocks per cluster with which three blocks of 256
 // threads share an SM, else two of 512; then the most groups that leave enough
 // blocks for the GPU.  0: none (the sample is too large, or its rows do not
-// divide into packs).
+// divide into packs).  Clusters of more than two pay off forward only (16x4096x512
+// bf16: 44 us in clusters, 51 in tiles; backward 109 and 87).
 static size_t gn_resident_plan(GnArgs* a, size_t eb, int V, bool backward) {
   if (V != 16 / (int)eb || a->S >= (1ll << 31) / ((int64_t)a->G * 8)) return 0;
   const int64_t unit = V / gn_gcd(a->cg, V);  // groups that make whole packs
   for (int T : {256, 512}) {
     const size_t most = T == 256 ? 74 * 1024 : 112 * 1024;
-    for (int split = 1; split <= 8; split *= 2) {
+    for (int split = 1; split <= (backward ? 2 : 8); split *= 2) {
       int64_t best = 0;
       for (int64_t n = ceil_div(a->G, unit); n >= 1; --n) {
         const int64_t k = min64(n * unit, a->G);
