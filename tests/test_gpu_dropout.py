@@ -6,7 +6,7 @@ import torch
 
 from spikestack_lite_b200 import ops
 from spikestack_lite_b200._lib import EngineError
-from tests.temporal_ref import U, assert_within, dropout_words, stored
+from tests.temporal_ref import U, assert_within, dropout_words, philox, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -115,6 +115,26 @@ def test_a_captured_graph_takes_the_keys_of_its_replay():
     key[1] += 1
     with pytest.raises(RuntimeError):
         torch.autograd.grad(out, xd, gy)
+
+
+def test_offsets_beyond_32_bits():
+    n = (1 << 31) + 6
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = ops.dropout(x, 0.5, (9, 1 << 35))
+    for start in (0, (1 << 31) - 8, n - 10):
+        first = start // 4
+        words = []
+        for i in range(first, first + 4):
+            words += philox((i & 0xFFFFFFFF, i >> 32, 0, (1 << 35) >> 32), (9, 0))
+        keep = torch.tensor([w >= 1 << 31 for w in words])[start - 4 * first:][:min(10, n - start)]
+        assert torch.equal(y[start:start + len(keep)].float().cpu(), 2.0 * keep.float())
+
+
+def test_no_second_derivative():
+    x = torch.randn(8, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(ops.dropout(x, 0.5, (0, 0)).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
 
 
 def test_refusals():

@@ -135,6 +135,34 @@ def test_parameter_gradients_are_the_same_bits_every_run():
         assert all(torch.equal(p, q) for p, q in zip(r, runs[0]))
 
 
+@pytest.mark.parametrize("shape", [(300, 300, 64, 4), (2, 900, 256, 8), (3, 1500, 96, 2), (40, 700, 40, 4)])
+def test_samples_in_clusters_and_in_tiles(shape):
+    # sizes at which the blocks of a cluster share a sample, forward, backward or both
+    S, P, C, G = shape
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w, b, gy = make(S, P, C, dtype, seed=P)
+        check(x, G, w, b, gy, "silu")
+
+
+def test_offsets_beyond_32_bits():
+    # 2.3e9 elements: one row pattern repeated, whose group statistics are those of the row
+    P, C, G = 70000, 33024, 4
+    row = torch.randn(C, generator=torch.Generator().manual_seed(3)).bfloat16()
+    x = row.cuda().expand(1, P, C).contiguous()
+    y = ops.group_norm_act(x, G)
+    ref = GroupNorm(row.view(1, 1, C), G, None, None, 1e-5, "none")
+    # the mean of P equal rows: their sums take log2(P) + 128 roundings more
+    for t in (0, 65535, P - 1):
+        assert_within(y[:, t:t + 1], ref.y, stored(2 * ref.y_err, ref.y, torch.bfloat16), f"row {t}")
+
+
+def test_no_second_derivative():
+    x = torch.randn(2, 5, 8, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(ops.group_norm_act(x, 2, act="silu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 @pytest.mark.parametrize("shape", [(3, 64, 128, 8), (2, 3000, 512, 32)])
 def test_runs_on_a_side_stream_and_in_a_graph(shape):
     S, P, C, G = shape

@@ -223,6 +223,56 @@ def test_non_finite_gates(L, dtype, form):
         assert h[0, L // 2, 2] == x[0, L // 2, 2] and h[1, 0, 3] == state[1, 3].to(DT[dtype])
 
 
+def test_lengths_of_planes_and_one_sided_gradients():
+    # (T, B, N, d) over dim 0 with a length per (b, n); gradients of x alone, of the gate alone
+    x, gate, state, gh, glast = make(6, 33, 20, "leaky", torch.float32, seed=11)
+    lengths = torch.tensor([0, 33, 5, 1, 32, 17])
+    ref = Recurrence(x, gate, state, "leaky", lengths, gh, glast)
+    view = lambda t: t.view(2, 3, 33, 20).movedim(2, 0).contiguous().cuda()  # noqa: E731
+    back = lambda t: t.movedim(0, 2).reshape(6, 33, 20)  # noqa: E731
+    xs, gs, ss = view(x), view(gate), state.view(2, 3, 20).cuda()
+    for mine, want, err in ((xs, ref.dx, ref.dx_err), (gs, ref.dgate, ref.dgate_err)):
+        mine.requires_grad_()
+        h, last = ops.gated_recurrence(xs, gs, ss, dim=0, lengths=lengths.view(2, 3).cuda())
+        assert_within(back(h), ref.h, stored(ref.h_err, ref.h, torch.float32), "h")
+        (got,) = torch.autograd.grad((h, last), mine, (view(gh), glast.view(2, 3, 20).cuda()))
+        assert_within(back(got), want, stored(err, want, torch.float32), "gradient")
+        mine.requires_grad_(False)
+    # x as its own gate: both gradients arrive
+    x.requires_grad_(False)
+    both = x.cuda().requires_grad_()
+    h, last = ops.gated_recurrence(both, both, state.cuda())
+    (got,) = torch.autograd.grad((h, last), both, (gh.cuda(), glast.cuda()))
+    own = Recurrence(x, x, state, "leaky", None, gh, glast)
+    assert_within(got, own.dx + own.dgate, own.dx_err + own.dgate_err + 2.0 ** -23 * (own.dx.abs() + own.dgate.abs()),
+                  "x as its own gate")
+
+
+def test_no_second_derivative():
+    x = torch.randn(2, 5, 8, device="cuda", requires_grad=True)
+    h, _ = ops.gated_recurrence(x, x)
+    (g,) = torch.autograd.grad(h.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    # 2.3e9 elements: the inputs broadcast along time, the states written out; constant gates have a closed form
+    L, D = 70000, 33000
+    g = torch.Generator().manual_seed(12)
+    x, gate, state = (torch.randn(1, D, generator=g) for _ in range(3))
+    gate = (gate + 6).bfloat16()
+    x = x.bfloat16()
+    h, last = ops.gated_recurrence(x.cuda().expand(1, L, D), gate.cuda().expand(1, L, D), state.cuda())
+    a = torch.sigmoid(gate.double())
+    for t in (0, 1000, 65535, L - 1):
+        want = a ** (t + 1) * state.double() + (1 - a ** (t + 1)) * x.double()
+        # a memory of 1 / (1 - a) steps, each off by a few u of the state: (see Recurrence)
+        err = 40 * 2.0 ** -24 * (1 / (1 - a)).clamp(max=t + 1) * (state.abs() + x.abs()).double()
+        assert_within(h[:, t], want, stored(err, want, torch.bfloat16), f"step {t}")
+    assert_within(last, want, err, "last")
+
+
 def test_runs_on_a_side_stream_and_in_a_graph():
     x, gate, state, gh, glast = make(2, 300, 64, "leaky", torch.float32, seed=1)
     x, gate, state, gh, glast = (t.cuda() for t in (x, gate, state, gh, glast))
