@@ -9,7 +9,9 @@
 //
 // Bound: HBM for fp32 (2 or 3 tensors moved once); for 16-bit elements the
 // generator's integer multiplies come close to it (14 32x32->64 products per
-// four elements), which is why it runs 7 rounds and not 10.
+// four elements), which is why it runs 7 rounds and not 10.  Measured on
+// 262144x512 bf16: 133 us with the residual (92 % of the time its bytes need at
+// the measured HBM rate), 106 us without (78 %, the generator).
 #include "elem.cuh"
 
 namespace spk {
@@ -75,7 +77,9 @@ __device__ __forceinline__ Pack<E, V> dropout_pack(const Pack<E, V>& x, const Pa
 // A thread takes U packs of V = 4 or 8 consecutive elements (16 bytes, V / 4
 // counters) at a time.  ALIGNED: every tensor is 16-byte aligned and the
 // accesses are 16 bytes wide; otherwise they are single elements, of the same
-// counters.  The last, partial pack goes by elements too.
+// counters.  The last, partial pack goes by elements too.  U = 2 once every
+// thread of a full GPU has a pack (262144x512 bf16 forward + backward 311 us with
+// one pack in flight, 240 with two), 1 below, to spread few packs.
 template <typename E, bool RES, bool ALIGNED, int U>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(DropoutArgs a) {
   constexpr int V = 16 / (int)sizeof(E);

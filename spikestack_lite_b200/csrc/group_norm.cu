@@ -11,7 +11,15 @@
 // (slope 10).  The variance is never a difference of two large sums: parts
 // carry (count, mean, sum of squares about their own mean) and are merged.
 //
-// Bound: HBM; x (and gy) read and y (dx) written.
+// Bound: HBM, x (and gy) read and y (dx) written, for fp32; the issue of
+// instructions (two for the MUFU unit among some 20 per element and pass with
+// SiLU) for 16-bit tensors.  Two forms.  Resident: a block or a cluster keeps
+// what it normalises in shared memory and every tensor crosses HBM once.
+// Tiled: samples beyond that pass twice, sums first.  Measured, SiLU:
+//   resident  256x1024x512 fp32 forward 178 us (92 % of the time its bytes need at
+//             the measured HBM rate), backward 387 us (64 %); bf16 117 / 269 us
+//   tiled     4x32768x512 bf16 93 us forward, 149 us backward (66 and 69 % of the
+//             bytes of both passes)
 #include "elem.cuh"
 
 namespace spk {
@@ -178,16 +186,16 @@ struct GnShare {
   int g0, ng;     // groups
 
   __device__ __forceinline__ explicit GnShare(const GnArgs& a) {
-    const int64_t unit = (int64_t)blockIdx.x / a.split;
+    const unsigned unit = blockIdx.x / (unsigned)a.split, sample = unit / (unsigned)a.tiles;  // below 2^31
     rank = (int)(blockIdx.x - unit * a.split);
-    s = unit / a.tiles;
-    g0 = (int)(unit - s * a.tiles) * a.k;
+    s = sample;
+    g0 = (int)(unit - sample * a.tiles) * a.k;
     ng = min(a.k, a.G - g0);
     p0 = (int64_t)rank * a.rows;
     P = positions(a, rank);
   }
   __device__ __forceinline__ static int positions(const GnArgs& a, int rank) {
-    return (int)max64(min64(a.P - (int64_t)rank * a.rows, a.rows), 0);
+    return max(min((int)a.P - rank * a.rows, a.rows), 0);  // split * rows < P + split
   }
 };
 
@@ -203,7 +211,7 @@ struct GnPacks {
     for (int i = 0; i < rows; ++i, p += step, to += blockDim.x * V)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(p) : "memory");
   }
-  __device__ __forceinline__ Pack<E, V> get(int i) const { return load_pack<E, V>(slot + (size_t)i * blockDim.x * V); }
+  __device__ __forceinline__ Pack<E, V> get(int i) const { return load_pack<E, V>(slot + i * (int)(blockDim.x * V)); }
 };
 __device__ __forceinline__ void gn_wait_packs() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -365,21 +373,24 @@ __global__ void __launch_bounds__(512, 2) gn_resident_backward_kernel(GnArgs a) 
   const int width = h.ng * a.cg;
   GnSpot q = gn_spot(V, a.tpr, a.rpp);
   q.live = q.live && q.cv < width;
-  const int rows = q.live ? (int)ceil_div(max(h.P - q.r, 0), a.rpp) : 0, c0 = h.g0 * a.cg + q.cv;
+  const int rows = q.live ? (max(h.P - q.r, 0) + a.rpp - 1) / a.rpp : 0, c0 = h.g0 * a.cg + q.cv;
   const int64_t at = (h.s * a.P + h.p0 + q.r) * a.C + c0, step = (int64_t)a.rpp * a.C;
   const GnPacks<E, V> x(gn_smem, rows), gy(gn_smem + a.held / 2, rows);
   x.ask(static_cast<const E*>(a.x) + at, step);
   gy.ask(static_cast<const E*>(a.gy) + at, step);
-  float2* const part = reinterpret_cast<float2*>(gn_smem + a.held);  // [rpp][width] sums of dz and dz xhat
-  float2* const sums = part + a.rpp * a.k * a.cg;                    // [width]
+  // where a warp holds whole rows, its lanes first add up theirs
+  const bool fold = 32 % a.tpr == 0;
+  const int sets = fold ? (int)blockDim.x / 32 : a.rpp;
+  float2* const part = reinterpret_cast<float2*>(gn_smem + a.held);  // [sets][width] sums of dz and dz xhat
+  float2* const sums = part + sets * a.k * a.cg;                     // [width]
   float2* const coef = sums + a.k * a.cg;                            // [k]
   GnAffine<V, M> f;
   if (q.live) gn_affine<V, M>(a, h.s, c0, &f);
   gn_wait_packs();
-  if (q.live) {
-    float s1[V], s2[V];
+  float s1[V], s2[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
+  for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.0f;
+  if (q.live) {
 #pragma unroll 2
     for (int i = 0; i < rows; ++i) {
       const Pack<E, V> xv = x.get(i), gv = gy.get(i);
@@ -392,12 +403,25 @@ __global__ void __launch_bounds__(512, 2) gn_resident_backward_kernel(GnArgs a) 
       }
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      part[q.r * width + q.cv + j] = make_float2(s1[j], s2[j] * f.rstd[M > 1 ? j : 0]);
+    for (int j = 0; j < V; ++j) s2[j] *= f.rstd[M > 1 ? j : 0];
+  }
+  if (fold) {
+    for (int o = a.tpr; o < 32; o *= 2) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s1[j] += __shfl_xor_sync(0xffffffffu, s1[j], o);
+        s2[j] += __shfl_xor_sync(0xffffffffu, s2[j], o);
+      }
+    }
+  }
+  if (q.live && (!fold || (int)(threadIdx.x & 31) < a.tpr)) {
+    float2* const to = part + (fold ? (int)threadIdx.x / 32 : q.r) * width + q.cv;
+#pragma unroll
+    for (int j = 0; j < V; ++j) to[j] = make_float2(s1[j], s2[j]);
   }
   __syncthreads();
   float2* const own = coef + a.k;  // [k] this block's sums of dn and dn xhat
-  gn_channel_sums(part, a.rpp, width, own + a.k, sums);
+  gn_channel_sums(part, sets, width, own + a.k, sums);
   const int lane = threadIdx.x & 31;
   const float inv = 1.0f / ((float)a.P * (float)a.cg);
   for (int g = threadIdx.x >> 5; g < h.ng; g += blockDim.x / 32) {
@@ -460,8 +484,9 @@ struct GnTile {
 template <int V>
 __device__ __forceinline__ GnTile gn_tile(const GnArgs& a, int64_t tile, const GnSpot& q) {
   GnTile t;
-  t.s = tile / a.tiles;
-  t.p0 = (tile - t.s * a.tiles) * a.rows;
+  const unsigned at = (unsigned)tile, sample = at / (unsigned)a.tiles;  // below 2^31
+  t.s = sample;
+  t.p0 = (int64_t)(at - sample * a.tiles) * a.rows;
   t.rows = (int)min64(a.rows, a.P - t.p0);
   t.c0 = (int)blockIdx.y * a.tpr * V + q.cv;
   t.live = q.live && t.c0 < a.C;
@@ -518,10 +543,10 @@ __global__ void __launch_bounds__(kGnThreads, 4) gn_stats_kernel(GnArgs a) {
   const int width = min(a.tpr * V, a.C - (int)blockIdx.y * a.tpr * V);
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
     float2 v = part[c];
-    float cnt = (float)(int)ceil_div(t.rows, a.rpp);
+    float cnt = (float)((t.rows + a.rpp - 1) / a.rpp);
     for (int r = 1; r < a.rpp && r < t.rows; ++r) {
       const float2 o = part[r * a.tpr * V + c];
-      const float k = (float)(int)ceil_div(t.rows - r, a.rpp), w = __fdividef(k, cnt + k), d = o.x - v.x;
+      const float k = (float)((t.rows - r + a.rpp - 1) / a.rpp), w = __fdividef(k, cnt + k), d = o.x - v.x;
       v.x = fmaf(d, w, v.x);
       v.y += fmaf(d * d, cnt * w, o.y);
       cnt += k;
@@ -563,7 +588,8 @@ __global__ void __launch_bounds__(kGnThreads) gn_stats_finish_kernel(GnArgs a) {
   __shared__ float sm[kGnThreads / 32];
   grid_dependents_may_start();
   grid_wait_for_previous();
-  const int64_t u = blockIdx.x, s = u / a.G, g = u - s * a.G;
+  const unsigned u = blockIdx.x, sample = u / (unsigned)a.G;
+  const int64_t s = sample, g = u - sample * a.G;
   const float2* part = reinterpret_cast<const float2*>(a.part) + s * a.tiles * a.C + g * a.cg;
   const float total = (float)a.P * (float)a.cg, rows = (float)a.rows;
   const float tail = (float)(int)(a.P - (int64_t)(a.tiles - 1) * a.rows);  // rows of the last tile
@@ -664,7 +690,8 @@ __global__ void __launch_bounds__(kGnThreads) gn_grad_finish_kernel(GnArgs a) {
   __shared__ float sm[kGnThreads / 32];
   grid_dependents_may_start();
   grid_wait_for_previous();
-  const int64_t u = blockIdx.x, s = u / a.G, g = u - s * a.G;
+  const unsigned u = blockIdx.x, sample = u / (unsigned)a.G;
+  const int64_t s = sample, g = u - sample * a.G;
   const float2* part = reinterpret_cast<const float2*>(a.part) + s * a.tiles * a.C + g * a.cg;
   const float* weight = a.weight != nullptr ? a.weight + g * a.cg : nullptr;
   float s1 = 0.0f, s2 = 0.0f;
@@ -770,7 +797,7 @@ static size_t gn_resident_layout(GnArgs* a, int V, int k, int T, int split, bool
   const double held = (double)ceil_div(a->rows, a->rpp) * T * 16 * (backward ? 2 : 1);
   if (held > most) return 0;
   a->held = (int)held;
-  const int parts = a->rpp * (int)width;
+  const int sets = backward && 32 % a->tpr == 0 ? T / 32 : a->rpp, parts = sets * (int)width;
   const size_t rest = backward ? (size_t)parts + width + 2 * k + T : (size_t)parts / (a->cg % V == 0 ? V : 1) + 2 * k;
   const size_t smem = a->held + rest * sizeof(float2);
   return smem <= most ? smem : 0;
@@ -780,14 +807,15 @@ static size_t gn_resident_layout(GnArgs* a, int V, int k, int T, int split, bool
 // (or whole ones); the fewest blocks per cluster with which three blocks of 256
 // threads share an SM, else two of 512; then the most groups that leave enough
 // blocks for the GPU.  0: none (the sample is too large, or its rows do not
-// divide into packs).  Clusters of more than two pay off forward only (16x4096x512
-// bf16: 44 us in clusters, 51 in tiles; backward 109 and 87).
+// divide into packs).  Clusters against tiles, us: forward 16x4096x512 bf16 44
+// and 51, 5x3001x320 bf16 11 and 21; backward 16x4096x512 bf16 86 and 86,
+// 16x2048x512 fp32 62 and 74, 5x3001x320 bf16 17 and 22.
 static size_t gn_resident_plan(GnArgs* a, size_t eb, int V, bool backward) {
   if (V != 16 / (int)eb || a->S >= (1ll << 31) / ((int64_t)a->G * 8)) return 0;
   const int64_t unit = V / gn_gcd(a->cg, V);  // groups that make whole packs
   for (int T : {256, 512}) {
     const size_t most = T == 256 ? 74 * 1024 : 112 * 1024;
-    for (int split = 1; split <= (backward ? 2 : 8); split *= 2) {
+    for (int split = 1; split <= 8; split *= 2) {
       int64_t best = 0;
       for (int64_t n = ceil_div(a->G, unit); n >= 1; --n) {
         const int64_t k = min64(n * unit, a->G);
