@@ -11,7 +11,7 @@
 // generator's integer multiplies come close to it (14 32x32->64 products per
 // four elements), which is why it runs 7 rounds and not 10.  Measured on
 // 262144x512 bf16: 133 us with the residual (92 % of the time its bytes need at
-// the measured HBM rate), 106 us without (78 %, the generator).
+// the measured HBM rate), 100 us without (82 %, the generator).
 #include "elem.cuh"
 
 namespace spk {
@@ -77,9 +77,10 @@ __device__ __forceinline__ Pack<E, V> dropout_pack(const Pack<E, V>& x, const Pa
 // A thread takes U packs of V = 4 or 8 consecutive elements (16 bytes, V / 4
 // counters) at a time.  ALIGNED: every tensor is 16-byte aligned and the
 // accesses are 16 bytes wide; otherwise they are single elements, of the same
-// counters.  The last, partial pack goes by elements too.  U = 2 once every
-// thread of a full GPU has a pack (262144x512 bf16 forward + backward 311 us with
-// one pack in flight, 240 with two), 1 below, to spread few packs.
+// counters.  The last, partial pack goes by elements too.  Once every thread of
+// a full GPU has a pack, U = 2 with a residual and 4 without (262144x512 bf16,
+// us: 155, 133 and 139 with one, two and four packs in flight; without a
+// residual 156, 106 and 100); below that 1, to spread few packs.
 template <typename E, bool RES, bool ALIGNED, int U>
 __global__ void __launch_bounds__(kDropThreads) dropout_kernel(DropoutArgs a) {
   constexpr int V = 16 / (int)sizeof(E);
@@ -133,7 +134,7 @@ static void dropout_launch(const DropoutArgs& a, bool aligned, cudaStream_t st) 
   else if (vecs <= most * kDropThreads)
     dropout_kernel<E, RES, true, 1><<<blocks, kDropThreads, 0, st>>>(a);
   else
-    dropout_kernel<E, RES, true, 2><<<blocks, kDropThreads, 0, st>>>(a);
+    dropout_kernel<E, RES, true, RES ? 2 : 4><<<blocks, kDropThreads, 0, st>>>(a);
 }
 
 }  // namespace spk

@@ -751,6 +751,7 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(GnArgs a) {
   const int c = blockIdx.x * 32 + threadIdx.x;
   float2 acc = make_float2(0.0f, 0.0f);
   if (c < a.C) {
+#pragma unroll 8
     for (int64_t r = threadIdx.y; r < a.parts; r += 32) {
       const float2 v = *reinterpret_cast<const float2*>(a.part + (r * a.C + c) * 2);
       acc.x += v.x;
