@@ -328,7 +328,8 @@ int spk_temporal_mean(const float* x, int T, int64_t B, int N, int d, float* mea
  * fp32 [B, D] contiguous: last = h_{len_b - 1} (the initial state for an
  * empty row).  lengths [B] int32 (null: all L; values are clamped to [0, L]):
  * inputs at t >= len_b are not read, and h is 0 there.  A NaN, or an
- * infinite x, makes the channel's later states non-finite.
+ * infinite x, makes the channel's later states non-finite; so does, in the gate
+ * form, a product of gates over up to 128 steps that overflows.
  * carry (optional, for the backward pass): fp32
  * [ceil(L / C) - 1, B, D] with C = spk_recurrence_chunk(dtype, B, L, D), the states
  * before each chunk of C steps but the first.  Arithmetic is fp32, h rounded once.  No reference

@@ -797,26 +797,41 @@ def gated_recurrence_step(x, gate, state, form="leaky", new_state=None):
     (contiguous float32; `state` itself updates it in place).  x and gate may be
     slices whose last dimension is contiguous.  Not differentiable."""
     what = "gated_recurrence_step"
-    dt = _checked(what, x, gate, state, new_state)
-    form = _form(form, what)
-    shape = x.shape
-    if gate.dtype != x.dtype or gate.shape != shape:
-        raise EngineError(f"{what}: gate must have x's shape and dtype")
-    if state.dtype != torch.float32 or state.shape != shape:
-        raise EngineError(f"{what}: state must be float32 of x's shape {tuple(shape)}")
-    if _wants_grad(x, gate, state):
-        raise EngineError(f"{what}: no backward pass (use gated_recurrence, or torch.no_grad())")
-    if not shape:
-        raise EngineError(f"{what}: x must have a channel dimension")
-    if new_state is not None and (new_state.dtype != torch.float32 or new_state.shape != shape
-                                  or not new_state.is_contiguous()):
-        raise EngineError(f"{what}: new_state must be contiguous float32 of x's shape {tuple(shape)}")
+    # one chain of cheap tests for the call that is right (a stream makes it per
+    # plane); what is wrong is looked for only when it fails
+    try:
+        shape = x.shape
+        dt, fm, dev = _DTYPES[x.dtype], _FORMS[form], x.get_device()
+        right = (dev >= 0 and gate.dtype == x.dtype and gate.shape == shape and gate.get_device() == dev
+                 and state.dtype == torch.float32 and state.shape == shape and state.get_device() == dev
+                 and (new_state is None or (new_state.dtype == torch.float32 and new_state.shape == shape
+                                            and new_state.get_device() == dev and new_state.is_contiguous()))
+                 and len(shape) > 0 and not _wants_grad(x, gate, state))
+    except (AttributeError, KeyError, TypeError):
+        right = False
+    if not right:
+        _checked(what, x, gate, state, new_state)
+        _form(form, what)
+        if gate.dtype != x.dtype or gate.shape != x.shape:
+            raise EngineError(f"{what}: gate must have x's shape and dtype")
+        if state.dtype != torch.float32 or state.shape != x.shape:
+            raise EngineError(f"{what}: state must be float32 of x's shape {tuple(x.shape)}")
+        if _wants_grad(x, gate, state):
+            raise EngineError(f"{what}: no backward pass (use gated_recurrence, or torch.no_grad())")
+        if not x.shape:
+            raise EngineError(f"{what}: x must have a channel dimension")
+        raise EngineError(f"{what}: new_state must be contiguous float32 of x's shape {tuple(x.shape)}")
     D = shape[-1]
-    (x, xs), (gate, gs), state = _rows(x), _rows(gate), _contig(state)
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if x.is_contiguous():
+        out, xs = torch.empty_like(x), D
+    else:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        x, xs = _rows(x)
+    gate, gs = (gate, D) if gate.is_contiguous() else _rows(gate)
+    state = _contig(state)
     if new_state is None:
         new_state = torch.empty_like(state)
-    _call(x, "spk_recurrence_step", x.data_ptr(), xs, gate.data_ptr(), gs, dt, form, x.numel() // D if D else 0, D,
+    _call(x, "spk_recurrence_step", x.data_ptr(), xs, gate.data_ptr(), gs, dt, fm, out.numel() // D if D else 0, D,
           state.data_ptr(), out.data_ptr(), new_state.data_ptr())
     return out, new_state
 
