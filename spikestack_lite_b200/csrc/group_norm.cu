@@ -817,7 +817,8 @@ static size_t gn_resident_plan(GnArgs* a, size_t eb, int V, bool backward) {
     const size_t most = T == 256 ? 74 * 1024 : 112 * 1024;
     for (int split = 1; split <= 8; split *= 2) {
       int64_t best = 0;
-      for (int64_t n = ceil_div(a->G, unit); n >= 1; --n) {
+      const int64_t widest = max64((int64_t)T * V / (unit * a->cg), 1);  // a row of packs, one per thread
+      for (int64_t n = min64(ceil_div(a->G, unit), widest); n >= 1; --n) {
         const int64_t k = min64(n * unit, a->G);
         if (k < a->G && k * a->cg * (int64_t)eb < 64) break;
         if (gn_resident_layout(a, V, (int)k, T, split, backward, most) == 0) continue;

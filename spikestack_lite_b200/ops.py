@@ -689,7 +689,14 @@ def _time_major(t, dim):
 def _empty_time(t, dim):
     """An uninitialised tensor of t's shape whose batch dimensions flatten, and its strides."""
     out = torch.empty_like(t, memory_format=torch.contiguous_format)
-    return _time_major(out, dim) if out.numel() else (out, (0, 0))
+    st = _time_strides(out, dim)
+    if st is None:  # time between the batch dimensions: laid out behind them
+        shape = list(t.shape)
+        steps = shape.pop(dim)
+        shape.insert(len(shape) - 1, steps)
+        out = t.new_empty(shape).movedim(-2, dim)
+        st = _time_strides(out, dim)
+    return out, st
 
 
 def _recurrence_forward(x, gate, state, form, dim, lengths, keep):

@@ -75,7 +75,8 @@ class GatedRecurrence(nn.Module):
 
     def _inputs(self, planes):
         """Values and gates (halves of one projection) of planes (P, N, d)."""
-        u = ops.group_norm_act(planes, self.groups, self.norm_weight, self.norm_bias, self.eps, act="silu")
+        u = ops.group_norm_act(planes, self.groups, self.norm_weight.float(), self.norm_bias.float(), self.eps,
+                               act="silu")
         vg = _linear(self.vg_proj, u)
         return vg[..., :self.d_model], vg[..., self.d_model:]
 

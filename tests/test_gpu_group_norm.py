@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 SHAPES = [(1, 1, 1, 1), (3, 64, 128, 8), (2, 1, 32, 8), (5, 7, 33, 11), (2, 301, 330, 10), (1, 1000, 12, 3),
-          (7, 13, 96, 1), (2, 130, 64, 64), (3, 50, 520, 4), (1, 5000, 40, 5), (300, 3, 16, 2), (1, 40, 4112, 16),
+          (7, 13, 96, 1), (2, 130, 64, 64), (3, 50, 520, 4), (1, 5000, 40, 5), (300, 3, 16, 2), (1, 40, 4112, 16), (2, 3, 6000, 3000), (1, 5, 24576, 24576),
           (2, 2500, 256, 32)]
 
 

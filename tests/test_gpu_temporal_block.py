@@ -154,6 +154,25 @@ def test_block_dropout_in_the_model():
     assert torch.equal(out, ops.dropout(blk.ffn(blk.norm2(mid)), 0.4, (2, 0), residual=mid))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_block_in_16_bits(dtype):
+    torch.manual_seed(4)
+    m = GatedRecurrence(64, groups=4, dropout=0.1).cuda().to(dtype)
+    x = torch.randn(9, 2, 5, 64, device="cuda").to(dtype).requires_grad_()
+    y, s = m(x)
+    assert y.dtype == dtype and s.dtype == torch.float32
+    y.float().square().sum().backward()
+    assert all(p.grad is not None and p.grad.dtype == dtype and p.grad.isfinite().all() for p in m.parameters())
+    m.eval()
+    with torch.no_grad():
+        want, last = m(x.detach())
+        state = None
+        for t in range(9):
+            y, state = m.step(x[t].detach(), state)
+            # one rounding of the projections' 16-bit results may fall the other way: a step of y's type
+            assert (y - want[t]).abs().max() <= 4 * torch.finfo(dtype).eps * want.abs().max()
+
+
 def test_refusals_and_autocast_branch():
     m = GatedRecurrence(32, groups=4).cuda()
     for bad in (torch.zeros(2, 3, 32, device="cuda"), torch.zeros(1, 2, 3, 16, device="cuda")):

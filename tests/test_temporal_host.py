@@ -158,7 +158,7 @@ def test_python_ops_refuse_cpu_tensors(lib):
 
 
 def test_time_strides():
-    from spikestack_lite_b200.ops import _time_major, _time_strides
+    from spikestack_lite_b200.ops import _empty_time, _time_major, _time_strides
 
     x = torch.zeros(4, 3, 5, 8)  # (T, B, N, d)
     assert _time_strides(x, 0) == (8, 120)
@@ -169,7 +169,21 @@ def test_time_strides():
     assert _time_strides(x[:, 0], 0) == (8, 120)
     assert _time_strides(x[0, 0, 0].expand(3, 5, 8), 1) == (0, 0)
     t, st = _time_major(x, 1)
-    assert t.shape == x.shape and st == _time_strides(t, 1) == (24, 8)
+    assert t.shape == x.shape and st == _time_strides(t, 1) == (32 * 3 // 4, 8)
+    for shape in ((4, 3, 5, 8), (2, 70, 3, 32), (3, 1, 5, 8), (2, 3, 4, 5, 6), (7, 9, 2), (4, 2)):
+        for dim in range(len(shape) - 1):  # an output holds exactly the elements that its strides reach
+            x = torch.zeros(shape)
+            out, (step_b, step_t) = _empty_time(x, dim)
+            steps, width = shape[dim], shape[-1]
+            rows = x.numel() // (steps * width)
+            assert out.shape == x.shape and step_t >= width and (step_b >= width or rows == 1)
+            reach = (rows - 1) * step_b + (steps - 1) * step_t + width
+            assert reach == x.numel() == out.untyped_storage().nbytes() // 4
+            at = torch.arange(rows).view(-1, 1, 1) * step_b + torch.arange(steps).view(-1, 1) * step_t + torch.arange(width)
+            out.copy_(torch.arange(x.numel()).view(shape))
+            flat = torch.empty(x.numel()).set_(out.untyped_storage())
+            want = torch.arange(x.numel()).view(shape).movedim(dim, -2).reshape(rows, steps, width)
+            assert torch.equal(flat[at.reshape(-1)].long(), want.reshape(-1))
 
 
 def test_modules_on_the_host():
