@@ -4,6 +4,7 @@ Every op validates its tensors (CUDA, float32, contiguous where the kernel
 needs it), passes raw pointers and the current stream of the tensors' device
 to libspk_b200.so and raises ``EngineError`` (a RuntimeError) on any failure.
 """
+import functools
 import weakref
 
 import torch
@@ -656,11 +657,8 @@ def _form(form, what):
         raise EngineError(f"{what}: form must be one of {sorted(_FORMS)}, got {form!r}") from None
 
 
-def _time_strides(t, dim):
-    """(stride of the flattened batch, stride of time) of t with time at
-    dimension `dim` and every other dimension but the last one batch; None when
-    the batch dimensions do not flatten or the last one is not contiguous."""
-    shape, strides = t.shape, t.stride()
+@functools.lru_cache(maxsize=1024)
+def _flat_strides(shape, strides, dim):
     if shape[-1] > 1 and strides[-1] != 1:
         return None
     step, size = None, 1
@@ -675,6 +673,13 @@ def _time_strides(t, dim):
         else:
             size *= n
     return (step if step is not None else 0), strides[dim]
+
+
+def _time_strides(t, dim):
+    """(stride of the flattened batch, stride of time) of t with time at
+    dimension `dim` and every other dimension but the last one batch; None when
+    the batch dimensions do not flatten or the last one is not contiguous."""
+    return _flat_strides(t.shape, t.stride(), dim)
 
 
 def _time_major(t, dim):
@@ -739,7 +744,7 @@ class _GatedRecurrence(torch.autograd.Function):
             gh, (ghb, ght) = _time_major(gh, dim)
         glast = None if glast is None else _contig(glast)
         dx, (db, dt) = _empty_time(x, dim)
-        dgate, _ = _empty_time(x, dim)
+        dgate = torch.empty_like(dx)  # dense: the same strides
         dstate = torch.empty_like(state)
         _call(x, "spk_recurrence_backward", ptr(x), xb, xt, ptr(gate), gb, gt, ptr(gh), ghb, ght, _DTYPES[x.dtype],
               ctx.form, B, L, D, ptr(state), ptr(lengths), ptr(carry), ptr(glast), ptr(dx), ptr(dgate), db, dt,
