@@ -18,7 +18,8 @@
 //   4 planes of 65536x512 fp32          284 us, all of it
 //   64x2048x512  bf16  89 us forward (69 %), 163 us backward (63 %)
 //   4x32768x512  bf16 141 us forward (44 %), 239 us backward (43 %)
-//   4x32768x512  fp32 199 us forward (62 %), 352 us backward (58 %)
+//   4x32768x512  fp32 199 us forward (62 %), 354 us backward (58 %)
+//   64x2048x512  fp32 149 us forward (83 %), 289 us backward (71 %)
 #include "elem.cuh"
 
 namespace spk {
@@ -43,7 +44,8 @@ struct RecArgs {
 struct RecPlan {
   int64_t chains, groups;  // chains = B * groups of neighbouring channels
   int64_t tiles, chunks;   // blocks' tiles (short), tiles along time (long)
-  int wt, cols, cluster;   // warps along time (short); channels per chain; blocks per chain (long)
+  int wt, cols;            // warps along time (short); channels per chain
+  int steps, cluster;      // steps per warp, blocks per chain (long)
 };
 
 // Two neighbouring channels: sm_100 multiplies and adds fp32 numbers in pairs.
@@ -845,26 +847,41 @@ static bool rec_aligned(const void* p, size_t eb, int64_t stride_b, int64_t stri
   return aligned_to(p, 4 * eb) && stride_b % 4 == 0 && stride_t % 4 == 0;
 }
 
-// Channels per chain of a long recurrence, V = 4 or 2 per lane: 128 (tiles of
-// 64 steps) or 64 (tiles of 128 steps: twice the chains, half the joins).
-// Forward + backward, us, 128 against 64 channels:
-//   bf16  1x32768x512: 218 / 194   4x32768x512: 380 / 389   64x2048x512: 253 / 348
-//   fp32  4x32768x512: 746 / 550   16x8192x512: 707 / 520   64x2048x512: 535 / 495
-// (fp32's backward stages leave room for one block per SM beside 128-channel maps).
-static int rec_long_cols(int dtype, int64_t B, int64_t D) {
-  return dtype == SPK_F32 || B * ceil_div(D, 128) < 16 ? 64 : 128;
+// Shape of a long recurrence's tiles: 128 channels (V = 4 per lane) or 64 (V =
+// 2), 8 or 16 steps per warp.  64 channels are twice the chains, 16 steps half
+// the joins, and fp32's backward stages leave room for one block per SM beside
+// 128-channel maps.  Forward and backward (which share the steps per tile), us:
+//                          4 x 8        2 x 16       2 x 8
+//   bf16  1x32768x512      86 / 132     70 / 127     84 / 128
+//         4x32768x512     145 / 240    137 / 255    153 / 254
+//         64x2048x512      90 / 165    119 / 241    127 / 224
+//   fp32  4x32768x512     270 / 476    200 / 355    219 / 338
+//         64x2048x512     147 / 383    172 / 324    174 / 289
+struct RecShape {
+  int cols, steps;
+};
+
+static RecShape rec_long_shape(int dtype, int64_t B, int64_t D, bool backward) {
+  const int64_t chains = B * ceil_div(D, 128);
+  if (dtype == SPK_F32) {
+    if (chains < 64) return {64, 16};
+    return backward ? RecShape{64, 8} : RecShape{128, 8};
+  }
+  return chains < 16 ? RecShape{64, 16} : RecShape{128, 8};
 }
 
 static int64_t rec_chunk(int dtype, int64_t B, int64_t L, int64_t D) {
-  return L <= 64 ? 64 : 64 * (128 / rec_long_cols(dtype, B, D));
+  return L <= 64 ? 64 : kRecWarps * rec_long_shape(dtype, B, D, false).steps;
 }
 
 // Batch rows that follow one another like channels (no lengths, batch stride D
 // everywhere) become channels first, so that narrow rows share a warp.
-static RecPlan rec_plan(RecArgs* a, int dtype, bool merge) {
+static RecPlan rec_plan(RecArgs* a, int dtype, bool backward, bool merge) {
   RecPlan p{};
   const int64_t chunk = rec_chunk(dtype, a->B, a->L, a->D);
-  p.cols = a->L <= 64 ? 128 : rec_long_cols(dtype, a->B, a->D);
+  const RecShape shape = rec_long_shape(dtype, a->B, a->D, backward);
+  p.cols = a->L <= 64 ? 128 : shape.cols;
+  p.steps = shape.steps;
   if (merge && a->lengths == nullptr) {
     a->D *= a->B;
     a->B = 1;
@@ -922,8 +939,12 @@ static cudaError_t rec_occupancy(K* kernel, int V, size_t stages, RecOccupancy* 
 
 template <typename E, typename Form, int V, int S, bool ALIGNED, bool BACKWARD>
 static cudaError_t rec_launch_long(const RecArgs& a, const RecPlan& p, cudaStream_t st) {
-  auto* const kernel = BACKWARD ? recurrence_long_backward_kernel<E, Form, V, S, ALIGNED>
-                                : recurrence_long_kernel<E, Form, V, S, ALIGNED>;
+  auto* const kernel = [] {  // only the one that is launched is compiled
+    if constexpr (BACKWARD)
+      return &recurrence_long_backward_kernel<E, Form, V, S, ALIGNED>;
+    else
+      return &recurrence_long_kernel<E, Form, V, S, ALIGNED>;
+  }();
   const size_t stages = rec_stage_bytes<E, V, S, ALIGNED>(BACKWARD ? 3 : 2);
   static PerDevice<RecOccupancy> cache;  // one per kernel
   RecOccupancy occ;
@@ -960,12 +981,20 @@ static int rec_run(bool backward, int dtype, int form, bool aligned, const RecAr
     using E = decltype(e);
     with_form<E>(form, [&](auto f) {
       using F = decltype(f);
-      if (a.L > 64 && p.cols == 64)
+      if (a.L > 64 && p.cols == 64 && p.steps == 16) {
         rc = aligned ? rec_launch_long<E, F, 2, 16, true>(backward, a, p, st)
                      : rec_launch_long<E, F, 2, 16, false>(backward, a, p, st);
-      else if (a.L > 64)
-        rc = aligned ? rec_launch_long<E, F, 4, 8, true>(backward, a, p, st)
-                     : rec_launch_long<E, F, 4, 8, false>(backward, a, p, st);
+      } else if (a.L > 64) {
+        if constexpr (sizeof(E) != 4)
+          rc = aligned ? rec_launch_long<E, F, 4, 8, true>(backward, a, p, st)
+                       : rec_launch_long<E, F, 4, 8, false>(backward, a, p, st);
+        else if (backward)
+          rc = aligned ? rec_launch_long<E, F, 2, 8, true, true>(a, p, st)
+                       : rec_launch_long<E, F, 2, 8, false, true>(a, p, st);
+        else
+          rc = aligned ? rec_launch_long<E, F, 4, 8, true, false>(a, p, st)
+                       : rec_launch_long<E, F, 4, 8, false, false>(a, p, st);
+      }
       else if (a.L > 4)
         rc = aligned ? rec_launch_short<E, F, 8, true>(backward, a, p, st)
                      : rec_launch_short<E, F, 8, false>(backward, a, p, st);
@@ -1020,7 +1049,7 @@ extern "C" int spk_recurrence(const void* x, int64_t x_stride_b, int64_t x_strid
                        spk::rec_aligned(h, eb, h_stride_b, h_stride_t) && spk::aligned_to(state, 16) &&
                        spk::aligned_to(last, 16) && spk::aligned_to(carry, 16);
   cudaStream_t st = (cudaStream_t)stream;
-  const spk::RecPlan p = spk::rec_plan(&a, dtype, x_stride_b == D && g_stride_b == D && h_stride_b == D);
+  const spk::RecPlan p = spk::rec_plan(&a, dtype, false, x_stride_b == D && g_stride_b == D && h_stride_b == D);
   return spk::rec_run(false, dtype, form, aligned, a, p, st);
 }
 
@@ -1072,7 +1101,7 @@ extern "C" int spk_recurrence_backward(const void* x, int64_t x_stride_b, int64_
                        spk::aligned_to(glast, 16) && spk::aligned_to(carry, 16) && spk::aligned_to(dstate, 16);
   cudaStream_t st = (cudaStream_t)stream;
   const spk::RecPlan p = spk::rec_plan(
-      &a, dtype, x_stride_b == D && g_stride_b == D && d_stride_b == D && (gh == nullptr || gh_stride_b == D));
+      &a, dtype, true, x_stride_b == D && g_stride_b == D && d_stride_b == D && (gh == nullptr || gh_stride_b == D));
   return spk::rec_run(true, dtype, form, aligned, a, p, st);
 }
 

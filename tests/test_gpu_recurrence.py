@@ -42,7 +42,8 @@ def check(x, gate, state, gh, glast, form, lengths=None, ref=None):
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("form", ["leaky", "gate"])
 @pytest.mark.parametrize("shape", [(1, 1, 1), (3, 4, 128), (2, 7, 33), (2, 64, 130), (2, 65, 128), (1, 128, 4),
-                                   (5, 200, 36), (1, 1025, 256), (3, 513, 197), (40, 3, 12), (1, 9000, 8)])
+                                   (5, 200, 36), (1, 1025, 256), (3, 513, 197), (40, 3, 12), (1, 9000, 8),
+                                   (70, 150, 36), (33, 200, 130), (129, 67, 128)])
 def test_matches_float64(shape, form, dtype):
     check(*make(*shape, form, DT[dtype], seed=sum(shape)), form)
 
