@@ -7,6 +7,7 @@ import torch
 from spikestack_lite_b200 import ops
 from spikestack_lite_b200._lib import EngineError
 from spikestack_lite_b200.attention import AstrocyteHebbianBlock
+from spikestack_lite_b200.graphs import CapturedForward
 from spikestack_lite_b200.recurrence import Dropout, GatedRecurrence
 from spikestack_lite_b200.transformer import SpikingTransformer
 
@@ -152,6 +153,18 @@ def test_block_dropout_in_the_model():
     out = blk(z)
     mid = ops.dropout(blk.attn(blk.norm1(z)), 0.4, (1, 0), residual=z)
     assert torch.equal(out, ops.dropout(blk.ffn(blk.norm2(mid)), 0.4, (2, 0), residual=mid))
+
+
+def test_captured_inference_with_the_recurrence():
+    torch.manual_seed(5)
+    m = SpikingTransformer(input_dim=48, d_model=128, seq_len=16, n_repeats=70, temporal=True, use_spikeskip=True,
+                           expansion=4, dropout=0.2, use_recurrence=True).cuda().eval()
+    x = torch.randn(3, 16, 48, device="cuda")
+    with torch.no_grad():
+        fwd = CapturedForward(m, x)
+        for _ in range(2):
+            x = torch.randn(3, 16, 48, device="cuda")
+            assert torch.equal(fwd(x).clone(), m(x))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
